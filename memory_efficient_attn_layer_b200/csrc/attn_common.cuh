@@ -22,10 +22,12 @@ namespace mea {
 constexpr uint32_t kPolyPairsFwd = MEA_POLY_FWD;
 constexpr uint32_t kPolyPairsBwd = MEA_POLY_BWD;
 
-// exp2 of a pair, on the FMA pipe when `poly` (argument clamped at -127, where
-// the result is negligible next to the row's largest term) else on MUFU.
+// exp2 of a pair, on the FMA pipe when `poly` (argument clamped at -126, where
+// the result is negligible next to the row's largest term; one lower, and the
+// polynomial's 2^f just below 1 would take the exponent field past zero) else on
+// MUFU.
 __device__ __forceinline__ float2 exp2_pair(float2 t, bool poly) {
-  if (poly) return exp2_poly2(make_float2(fmaxf(t.x, -127.f), fmaxf(t.y, -127.f)));
+  if (poly) return exp2_poly2(make_float2(fmaxf(t.x, -126.f), fmaxf(t.y, -126.f)));
   return make_float2(ex2(t.x), ex2(t.y));
 }
 
