@@ -194,6 +194,48 @@ int mea_qk_norm_rope_backward(const mea_block_dims* d, const float* dq_acc, cons
 /* rms_norm_backward_new (fast_triton_attn.py:663-669): dx from d(xn), x and r. */
 int mea_rmsnorm_backward(int rows, int C, const void* dxn, const void* x, const float* r, void* dx, void* stream);
 
+/* ---------------------------------------------------------------- packed sequences
+ * No counterpart in the reference, whose attention takes equal lengths and one
+ * key/value head per query head.  Causal softmax attention over sequences of
+ * any lengths packed along one row axis, with grouped heads:
+ * q, o are [total, Hq, N], k, v are [total, Hkv, N], Hq a multiple of Hkv, and
+ * query head h reads key/value head h / (Hq / Hkv).  Sequence s owns rows
+ * cu_seqlens[s] .. cu_seqlens[s+1] (device int32, n_seqs + 1 values rising from
+ * >= 0 to <= total; a sequence may be empty).  Rows that no sequence owns are
+ * written as zeros in o, dq, dk and dv, and no value of theirs reaches another
+ * row.  If cu_seqlens does not rise, every output row is zero and the status
+ * word is set (kernel 4; mea_read_status reports MEA_ERR_INVALID_ARGUMENT).
+ *
+ * N is a multiple of 8 up to 128; dtype MEA_BF16 or MEA_FP16.  Row and head
+ * strides are in elements, multiples of 8 and at least N, with the N values of
+ * a head contiguous; o, dq, dk, dv are contiguous.
+ *
+ * A row's output depends on no later row and on no other sequence, also when
+ * those hold inf or NaN.  In the backward an inf or NaN stays within its own
+ * sequence but may reach any gradient of it.  Results do not depend on the
+ * order in which the GPU runs the tiles: the same call gives the same bits. */
+enum { MEA_BF16 = 0, MEA_FP16 = 1, MEA_FP32 = 2 };
+typedef struct mea_packed_dims {
+  int total, n_seqs, Hq, Hkv, N;
+  int dtype;
+  float scale; /* factor on q.k (1/sqrt(N) in the block) */
+  long long q_row, q_head, k_row, k_head, v_row, v_head;
+} mea_packed_dims;
+/* Bytes of the plan (the list of tiles) that the forward writes and the
+ * backward of the same call reads; 256-byte aligned device memory. */
+size_t mea_packed_plan_size(const mea_packed_dims* d);
+/* o = causal softmax(scale q k^T) v per sequence; lse2[total, Hq] (fp32 row
+ * log-sum-exp in log2 units) on the rows of sequences. */
+int mea_packed_attention_forward(const mea_packed_dims* d, const void* q, const void* k, const void* v,
+                                 const int* cu_seqlens, void* o, float* lse2, void* plan, size_t plan_bytes,
+                                 int* status, void* stream);
+/* dq, dk, dv of the same call from its o, lse2 and plan and from dO (strides
+ * as q's).  delta: fp32 [total, Hq] workspace. */
+int mea_packed_attention_backward(const mea_packed_dims* d, const void* q, const void* k, const void* v, const void* o,
+                                  const void* dO, long long do_row, long long do_head, const float* lse2,
+                                  const void* plan, size_t plan_bytes, float* delta, void* dq, void* dk, void* dv,
+                                  int* status, void* stream);
+
 /* ---------------------------------------------------------------- no allocation
  * No counterpart in the reference.  mea_attention_backward for callers that
  * cannot allocate device memory (for example a plugin whose execute callback

@@ -10,6 +10,7 @@ from .dp import allreduce_grads, overlap_grad_allreduce
 from .fused_attn import FusedAttentionFunction, fused_attn
 from .module import CausalSoftmaxAttention, Yarn
 from .optim import ShardedAdamW
+from .packed import PackedAttentionFunction, packed_attention
 
 __all__ = ["fused_attn", "FusedAttentionFunction", "CausalSoftmaxAttention", "Yarn", "allreduce_grads",
-           "overlap_grad_allreduce", "ShardedAdamW", "MeaError", "check_device_status"]
+           "overlap_grad_allreduce", "packed_attention", "PackedAttentionFunction", "ShardedAdamW", "MeaError", "check_device_status"]

@@ -28,6 +28,16 @@ class MeaBlockDims(ctypes.Structure):
                 ("N", ctypes.c_int), ("T_max", ctypes.c_int), ("eps", ctypes.c_float)]
 
 
+MEA_BF16, MEA_FP16, MEA_FP32 = 0, 1, 2
+DTYPE_CODES = {torch.bfloat16: MEA_BF16, torch.float16: MEA_FP16, torch.float32: MEA_FP32}
+
+
+class MeaPackedDims(ctypes.Structure):
+    _fields_ = [("total", ctypes.c_int), ("n_seqs", ctypes.c_int), ("Hq", ctypes.c_int), ("Hkv", ctypes.c_int),
+                ("N", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_float),
+                *[(f"{t}_{d}", ctypes.c_longlong) for t in "qkv" for d in ("row", "head")]]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _LL = ctypes.c_longlong
@@ -35,6 +45,7 @@ _F = ctypes.c_float
 _DB = ctypes.c_double
 _S = ctypes.c_size_t
 _D = ctypes.POINTER(MeaBlockDims)
+_PD = ctypes.POINTER(MeaPackedDims)
 
 # name -> (restype, argtypes); mirrors include/mea.h
 SIGNATURES = {
@@ -62,6 +73,9 @@ SIGNATURES = {
     "mea_qk_norm_rope_backward": (_I, [_D, _P, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P, _P, _P]),
     "mea_rmsnorm_backward": (_I, [_I, _I, _P, _P, _P, _P, _P]),
     "mea_attention_backward_noalloc": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P, _P]),
+    "mea_packed_plan_size": (_S, [_PD]),
+    "mea_packed_attention_forward": (_I, [_PD, _P, _P, _P, _P, _P, _P, _P, _S, _P, _P]),
+    "mea_packed_attention_backward": (_I, [_PD, _P, _P, _P, _P, _P, _LL, _LL, _P, _P, _S, _P, _P, _P, _P, _P, _P]),
     "mea_adamw_step": (_I, [_LL, _P, _P, _P, _P, _P, _DB, _DB, _DB, _DB, _DB, _F, _I, _P]),
     "mea_selftest_wait": (_I, [_P, ctypes.c_ulonglong, _I, _P]),
     "mea_profile_enable": (_I, [_I]),
@@ -186,7 +200,12 @@ def status_buffer(device: torch.device) -> torch.Tensor:
     return _watcher(device).word
 
 
+_KID_PACKED_PLAN = 4
+
+
 def _timeout_error(v: int, when: str) -> MeaError:
+    if (v >> 8) & 0xFF == _KID_PACKED_PLAN:
+        return MeaError(1, f"packed attention: cu_seqlens did not rise from >= 0 to <= total {when}")
     return MeaError(MEA_ERR_DEVICE_TIMEOUT, f"device wait timed out (kernel {(v >> 8) & 0xFF}, site "
                                             f"{(v >> 16) & 0xFFFF}) {when}")
 
@@ -203,6 +222,47 @@ def poll_status(device: torch.device) -> None:
     v = _watcher(device).take(block=False)
     if v != 0:
         raise _timeout_error(v, "in an earlier call")
+
+
+def status_word(device: torch.device) -> int:
+    """Address of the device's status word.  It is allocated by the first call on
+    the device, which must not be a captured one: the word would belong to that
+    graph's memory."""
+    if _device_index(device) not in _watch and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call on a device must come before a stream capture (it allocates the status word)")
+    return _watcher(device).word.data_ptr()
+
+
+def note_status_eager(device: torch.device) -> None:
+    """note_status, except in a stream capture: the event behind the copy would
+    belong to the graph, and a replay's error stays in the word until the next
+    eager call copies it."""
+    if not torch.cuda.is_current_stream_capturing():
+        _watcher(device).note()
+
+
+def poll_status_eager(device: torch.device) -> None:
+    """poll_status, except in a stream capture (an event query would end it)."""
+    if not torch.cuda.is_current_stream_capturing():
+        poll_status(device)
+
+
+class _SameDevice:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def on_device(device: torch.device):
+    """Context with `device` current; nothing is switched when it already is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 def check_device_status(device: torch.device | None = None) -> None:

@@ -392,6 +392,8 @@ int mea_read_status(const int* status_dev, int* out, void* stream) {
     return set_error(MEA_ERR_CUDA, "stream sync: %s", cudaGetErrorString(cudaGetLastError()));
   if (cudaMemcpy(out, status_dev, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
     return set_error(MEA_ERR_CUDA, "status copy failed");
+  if (*out != 0 && ((*out >> 8) & 0xFF) == KID_PACKED_PLAN)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: cu_seqlens must rise from >= 0 to <= total");
   if (*out != 0)
     return set_error(MEA_ERR_DEVICE_TIMEOUT, "device wait timed out (kernel %d, site %d)", (*out >> 8) & 0xFF,
                      (*out >> 16) & 0xFFFF);

@@ -1,0 +1,102 @@
+// What the packed-sequence attention kernels share: the work plan, element
+// types, tile geometry and masks.
+//
+// Layout.  q, o are [total, Hq, N]; k, v are [total, Hkv, N]; sequence s owns
+// rows cu[s] .. cu[s+1], and query head h reads key/value head h / G with
+// G = Hq / Hkv.  A query tile holds `tt` consecutive tokens of one sequence
+// times `p` neighbouring heads of one group (p divides G), token-major: tile
+// row r is token r / p, head r % p.  One 3-D TMA box {64 elements, p heads, tt
+// tokens} brings it in, so a group's heads share every K/V tile that is loaded
+// and a short sequence still fills rows of the 128-row MMA.
+//
+// Head dims up to 64 run as HD = 64 and up to 128 as HD = 128: TMA fills the
+// columns past N with zeros, which add nothing to a score or a product.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "attn_common.cuh"
+
+namespace mea {
+
+// ---- work plan (device memory, written by packed_plan_kernel) ----
+// header, then int4 items {first row of the sequence, its length, tile, 0}:
+// query tiles (cap_q) and 128-row key tiles (cap_k), each sorted by falling
+// work so that the tiles that take longest start first.
+struct PackedHeader {
+  int n_q, n_k;    // items of each kind
+  int first, end;  // rows [first, end) belong to sequences
+  int pad[4];
+};
+
+struct PackedDims {
+  int total, n_seqs, Hq, Hkv, N;
+  int p, tt;        // heads and tokens of a query tile
+  int cap_q, cap_k;
+  int hg;           // query tiles per token tile: Hq / p
+};
+
+struct PackedPlan {
+  const PackedHeader* head;
+  const int4* q_items;
+  const int4* k_items;
+};
+
+// ---- element types ----
+struct Bf16 {
+  static constexpr uint32_t FMT = 1;
+  static constexpr uint32_t EXP = 0x7F80;  // exponent field: all ones is inf or NaN
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+  __device__ static __forceinline__ float lo(uint32_t v) { return bf16_lo(v); }
+  __device__ static __forceinline__ float hi(uint32_t v) { return bf16_hi(v); }
+  // acc + 0 * v per half: stays 0 unless v holds an inf or NaN.
+  __device__ static __forceinline__ void probe(uint32_t& acc, uint32_t v) {
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
+  }
+};
+struct Fp16 {
+  static constexpr uint32_t FMT = 0;
+  static constexpr uint32_t EXP = 0x7C00;
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ float lo(uint32_t v) { return __half2float(__ushort_as_half(uint16_t(v))); }
+  __device__ static __forceinline__ float hi(uint32_t v) { return __half2float(__ushort_as_half(uint16_t(v >> 16))); }
+  __device__ static __forceinline__ void probe(uint32_t& acc, uint32_t v) {
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
+  }
+};
+template <class T>
+__device__ __forceinline__ bool half_nonfinite(uint32_t h) {
+  return (h & T::EXP) == T::EXP;
+}
+
+// ---- shared memory ----
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&w)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Rows [r0, 128) of a [128 x HD] tile (64-column chunks of 128-byte rows) to
+// zero, by one warp.  A whole row is cleared, so the swizzle does not matter.
+template <int HD>
+__device__ __forceinline__ void zero_rows(uint32_t tile, int r0, int lane) {
+  const int units = (128 - r0) * 8;
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c)
+    for (int u = lane; u < units; u += 32) sts128(tile + c * 16384 + r0 * 128 + u * 16, 0, 0, 0, 0);
+}
+
+// Rows of `width` 16-byte units outside [first, end) of a [total, width] output
+// to zero, spread over the grid: no sequence owns them.
+__device__ __forceinline__ void zero_outside(uint4* out, int total, int first, int end, long long width, int block,
+                                             int blocks, int thread, int threads) {
+  const int behind = total - end;
+  for (int r = block; r < first + behind; r += blocks) {
+    uint4* row = out + (long long)(r < first ? r : end + (r - first)) * width;
+    for (long long u = thread; u < width; u += threads) row[u] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+}  // namespace mea

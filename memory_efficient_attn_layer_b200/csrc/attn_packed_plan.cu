@@ -1,0 +1,258 @@
+// The work plan of the packed-sequence attention, and its host side: shapes,
+// strides, tensor maps and buffer sizes shared by the forward and backward.
+//
+// The lengths are device data, so the host only knows how many tiles there can
+// be: total / tt + n_seqs.  One block turns cu_seqlens into the list of tiles,
+// sorted by falling work (a counting sort over 1024 classes): the kernels then
+// start the longest tiles first, and blocks past the list's end leave at once.
+// The plan belongs to the call, never to a later one: a captured call builds it
+// again from the values cu_seqlens has at the replay.
+#include "attn_packed.h"
+#include "attn_packed.cuh"
+
+namespace mea {
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_CLASSES = 1024;
+constexpr int PLAN_SMEM_SEQS = 1024;  // prefix sums of up to this many sequences stay in shared memory
+
+// Exclusive block-wide prefix sum of one value per thread; *sum is the total.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // warp_sums of an earlier call are read
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = warp_sums[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  *sum = warp_sums[31];
+  return x - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+// Last index s with pre[s] <= id (pre is non-decreasing, pre[0] = 0): the
+// sequence that tile `id` lies in; sequences without tiles are passed over.
+__device__ __forceinline__ int seq_of(const int* pre, int n_seqs, int id) {
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= id)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __restrict__ cu, int n_seqs, int total,
+                                                                   int tt, int cap_q, int cap_k, PackedHeader* head,
+                                                                   int4* q_items, int4* k_items, int* scratch,
+                                                                   int* status) {
+  __shared__ int pre_s[2 * PLAN_SMEM_SEQS];
+  __shared__ int hist[PLAN_CLASSES];
+  __shared__ int warp_sums[32];
+  __shared__ int longest_s;
+  const int tid = threadIdx.x;
+  pdl_launch();
+  if (tid == 0) longest_s = 0;
+
+  // cu_seqlens must rise from >= 0 to <= total; otherwise no tile is made (every
+  // output row is then zero) and the status word says so.
+  bool good = true;
+  for (int i = tid; i < n_seqs; i += PLAN_THREADS) good &= cu[i] >= 0 && cu[i] <= cu[i + 1] && cu[i + 1] <= total;
+  if (!__syncthreads_and(good)) {
+    if (tid == 0) {
+      record_error(status, KID_PACKED_PLAN, 1);
+      *head = PackedHeader{0, 0, 0, 0, {0, 0, 0, 0}};
+    }
+    return;
+  }
+
+  int* pre_q = n_seqs <= PLAN_SMEM_SEQS ? pre_s : scratch;
+  int* pre_k = pre_q + (n_seqs <= PLAN_SMEM_SEQS ? PLAN_SMEM_SEQS : n_seqs);
+  int n_q = 0, n_k = 0, longest = 0;
+  for (int s0 = 0; s0 < n_seqs; s0 += PLAN_THREADS) {
+    const int s = s0 + tid;
+    const int len = s < n_seqs ? cu[s + 1] - cu[s] : 0;
+    longest = max(longest, len);
+    int sum_q, sum_k;
+    const int at_q = block_scan(int((long long)(len + tt - 1) / tt), warp_sums, &sum_q);
+    const int at_k = block_scan((len + 127) >> 7, warp_sums, &sum_k);
+    if (s < n_seqs) {
+      pre_q[s] = n_q + at_q;
+      pre_k[s] = n_k + at_k;
+    }
+    n_q += sum_q;
+    n_k += sum_k;
+  }
+  atomicMax(&longest_s, longest);
+  __syncthreads();
+  longest = longest_s;
+  if (tid == 0) *head = PackedHeader{min(n_q, cap_q), min(n_k, cap_k), cu[0], cu[n_seqs], {0, 0, 0, 0}};
+
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {  // query tiles, then key tiles
+    const int* pre = kind ? pre_k : pre_q;
+    const int n = kind ? n_k : n_q, cap = kind ? cap_k : cap_q;
+    int4* items = kind ? k_items : q_items;
+    const int most = kind ? (longest + tt - 1) / tt : (longest + 127) >> 7;  // steps of the longest tile
+    int shift = 0;
+    while ((most >> shift) >= PLAN_CLASSES) ++shift;
+    auto item = [&](int id, int& cls) {
+      const int s = seq_of(pre, n_seqs, id);
+      const int begin = cu[s], len = cu[s + 1] - begin, tile = id - pre[s];
+      // steps: key tiles up to the query tile's last token, or query tiles from the key tile's first
+      const int steps = kind ? (len + tt - 1) / tt - tile * 128 / tt
+                             : (int(min((long long)(tile + 1) * tt, (long long)len)) + 127) >> 7;
+      cls = (most >> shift) - (steps >> shift);
+      return make_int4(begin, len, tile, 0);
+    };
+    hist[tid] = 0;
+    __syncthreads();
+    for (int id = tid; id < n; id += PLAN_THREADS) {
+      int cls;
+      item(id, cls);
+      atomicAdd(&hist[cls], 1);
+    }
+    __syncthreads();
+    int all;
+    const int at = block_scan(hist[tid], warp_sums, &all);
+    __syncthreads();
+    hist[tid] = at;
+    __syncthreads();
+    for (int id = tid; id < n; id += PLAN_THREADS) {
+      int cls;
+      const int4 it = item(id, cls);
+      const int slot = atomicAdd(&hist[cls], 1);  // order within a class is free: tiles are independent
+      if (slot < cap) items[slot] = it;
+    }
+    __syncthreads();
+  }
+}
+static_assert(PLAN_CLASSES == PLAN_THREADS, "one class per thread in the scan");
+
+// ---------------------------------------------------------------- host side
+static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+int packed_dims(const mea_packed_dims* d, PackedDims* out) {
+  if (!d) return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: dims is NULL");
+  if (d->total < 0 || d->n_seqs < 0)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: total=%d and n_seqs=%d must be >= 0", d->total,
+                     d->n_seqs);
+  if (d->Hq <= 0 || d->Hkv <= 0 || d->Hq % d->Hkv)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: Hq=%d must be a positive multiple of Hkv=%d", d->Hq,
+                     d->Hkv);
+  if (d->N <= 0 || d->N > 128 || d->N % 8)
+    return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention: head dim N=%d must be a multiple of 8 up to 128", d->N);
+  if (d->dtype != MEA_BF16 && d->dtype != MEA_FP16)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: dtype %d is neither MEA_BF16 nor MEA_FP16", d->dtype);
+  if (!(d->scale > 0.f) || !(d->scale < 3.0e38f))
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: scale=%g must be positive and finite", d->scale);
+  PackedDims o;
+  o.total = d->total;
+  o.n_seqs = d->n_seqs;
+  o.Hq = d->Hq;
+  o.Hkv = d->Hkv;
+  o.N = d->N;
+  // Heads per query tile: the divisor of the group size that fills most of the
+  // 128 rows, the larger one at a tie (fewer K/V reads).
+  const int G = d->Hq / d->Hkv;
+  o.p = 1;
+  o.tt = 128;
+  for (int p = 2; p <= G && p <= 128; ++p)
+    if (G % p == 0 && p * (128 / p) >= o.p * o.tt) {
+      o.p = p;
+      o.tt = 128 / p;
+    }
+  o.hg = d->Hq / o.p;
+  const long long cap_q = (long long)d->total / o.tt + d->n_seqs, cap_k = (long long)d->total / 128 + d->n_seqs;
+  if (cap_q * o.hg > 0x7fffffffLL || cap_k * d->Hkv > 0x7fffffffLL)
+    return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention: total=%d rows, %d sequences and %d heads make too many tiles",
+                     d->total, d->n_seqs, d->Hq);
+  o.cap_q = int(cap_q);
+  o.cap_k = int(cap_k);
+  *out = o;
+  return MEA_OK;
+}
+
+size_t packed_plan_bytes(const PackedDims& d) {
+  return up256(sizeof(PackedHeader)) + up256(sizeof(int4) * size_t(d.cap_q)) + up256(sizeof(int4) * size_t(d.cap_k)) +
+         (d.n_seqs > PLAN_SMEM_SEQS ? up256(sizeof(int) * 2 * size_t(d.n_seqs)) : 0);
+}
+
+PackedPlan packed_plan_view(const PackedDims& d, const void* plan) {
+  const char* b = static_cast<const char*>(plan);
+  PackedPlan v;
+  v.head = reinterpret_cast<const PackedHeader*>(b);
+  b += up256(sizeof(PackedHeader));
+  v.q_items = reinterpret_cast<const int4*>(b);
+  b += up256(sizeof(int4) * size_t(d.cap_q));
+  v.k_items = reinterpret_cast<const int4*>(b);
+  return v;
+}
+
+int run_packed_plan(const PackedDims& d, const int* cu, void* plan, int* status, cudaStream_t st) {
+  const PackedPlan v = packed_plan_view(d, plan);
+  char* scratch = static_cast<char*>(plan) + up256(sizeof(PackedHeader)) + up256(sizeof(int4) * size_t(d.cap_q)) +
+                  up256(sizeof(int4) * size_t(d.cap_k));
+  packed_plan_kernel<<<1, PLAN_THREADS, 0, st>>>(cu, d.n_seqs, d.total, d.tt, d.cap_q, d.cap_k,
+                                                 const_cast<PackedHeader*>(v.head), const_cast<int4*>(v.q_items),
+                                                 const_cast<int4*>(v.k_items), reinterpret_cast<int*>(scratch), status);
+  return check_launch("packed_plan_kernel");
+}
+
+int packed_check_rows(const char* name, const void* base, long long tok, long long head, const PackedDims& d, int heads) {
+  if (!base) return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: %s is NULL", name);
+  if (reinterpret_cast<uintptr_t>(base) & 15)
+    return set_error(MEA_ERR_ALIGNMENT, "packed attention: %s must be 16-byte aligned", name);
+  if ((d.total > 1 && (tok < d.N || tok % 8)) || (heads > 1 && (head < d.N || head % 8)))
+    return set_error(MEA_ERR_ALIGNMENT,
+                     "packed attention: the row and head strides of %s (%lld, %lld) must be multiples of 8 elements, "
+                     "at least N=%d", name, tok, head, d.N);
+  if ((d.total > 1 && tok >= (1LL << 38)) || (heads > 1 && head >= (1LL << 38)))
+    return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention: a stride of %s is too large", name);
+  return MEA_OK;
+}
+
+int packed_map(CUtensorMap* map, const PackedDims& d, int dtype, const void* base, long long tok, long long head,
+               int heads, int box_heads, int box_rows) {
+  // The stride of a dimension of extent one is never used; it still has to be a legal one.
+  if (heads == 1) head = d.N;
+  if (d.total == 1) tok = (long long)heads * (head > d.N ? head : d.N);
+  return make_tmap_3d(map, base, uint64_t(d.N), uint64_t(heads), uint64_t(head) * 2, uint64_t(d.total),
+                      uint64_t(tok) * 2, 64, uint32_t(box_heads), uint32_t(box_rows), CU_TENSOR_MAP_SWIZZLE_128B,
+                      dtype == MEA_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+}
+
+cudaLaunchConfig_t packed_launch(int grid, int threads, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr->val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+}  // namespace mea
+
+extern "C" size_t mea_packed_plan_size(const mea_packed_dims* d) {
+  mea::PackedDims pd;
+  if (mea::packed_dims(d, &pd) != MEA_OK) return 0;
+  return mea::packed_plan_bytes(pd);
+}

@@ -22,7 +22,8 @@ namespace mea {
 // Layout of the 32-bit device status word: 0 = ok; otherwise
 //   bits 0..7 = 0x5A (marker), bits 8..15 = kernel id, bits 16..31 = wait site.
 enum KernelId : uint32_t {
-  KID_GEMM = 1, KID_ATTN_FWD = 2, KID_ATTN_BWD = 3, KID_TEST = 9,
+  KID_GEMM = 1, KID_ATTN_FWD = 2, KID_ATTN_BWD = 3, KID_PACKED_PLAN = 4, KID_PACKED_FWD = 5, KID_PACKED_DQ = 6,
+  KID_PACKED_DKV = 7, KID_TEST = 9,
 };
 
 __device__ __forceinline__ void record_error(int* status, uint32_t kid, uint32_t site) {
@@ -136,6 +137,12 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Programmatic dependent launch: wait until the kernels this launch depends on
+// have completed and their writes are visible (no effect in a plain launch);
+// let the next kernel of the stream start its prologue.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ----------------------------------------------------------------------------
 // TMA (bulk tensor copies).  Tensor maps are __grid_constant__ kernel params.
 // ----------------------------------------------------------------------------
@@ -146,6 +153,11 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
 // Plain (non-tensor) bulk copy global -> shared; dst, src 16-byte aligned, bytes % 16 == 0.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -402,6 +414,11 @@ __host__ __device__ constexpr uint32_t idesc_bf16(uint32_t M, uint32_t N, uint32
          | ((M >> 4) << 24);  // M / 16
 }
 
+// The same for fp16 (fmt 0) or bf16 (fmt 1) operands; A and B share the type.
+__host__ __device__ constexpr uint32_t idesc_16bit(uint32_t fmt, uint32_t M, uint32_t N, uint32_t a_mn, uint32_t b_mn) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
 // Instruction descriptor for kind::f8f6f4 with e4m3 A and B (format code 0),
 // fp32 D, both operands K-major, M x N tile.
 __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t M, uint32_t N) {
@@ -420,6 +437,12 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float max3f(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The same, NaN if any input is.
+__device__ __forceinline__ float max3f_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // Packed fp32 pair arithmetic (sm_100+): one instruction for two lanes of work.

@@ -17,6 +17,11 @@ int make_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t ou
                  uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle,
                  CUtensorMapDataType dtype = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
 
+// Encodes a 3-D tiled tensor map of 16-bit elements: `inner` contiguous
+// elements, then n1 and n2 with byte strides s1 and s2 (multiples of 16).
+int make_tmap_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t n1, uint64_t s1, uint64_t n2, uint64_t s2,
+                 uint32_t box0, uint32_t box1, uint32_t box2, CUtensorMapSwizzle swizzle, CUtensorMapDataType dtype);
+
 // Swizzle mode for a row of `row_bytes` bytes in shared memory (32, 64 or 128).
 inline CUtensorMapSwizzle swizzle_for(uint32_t row_bytes) {
   return row_bytes >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B
