@@ -264,6 +264,54 @@ int mea_adamw_step(long long n, float* master, float* exp_avg, float* exp_avg_sq
                    void* param_bf16, double lr, double beta1, double beta2, double eps, double weight_decay,
                    float grad_scale, int step, void* stream);
 
+/* mea_adamw_step with the gradient clipped by its global norm: sumsq (device
+ * fp64) is the sum of squares of every gradient before grad_scale, over all
+ * shards and ranks (mea_grad_norm, then the caller's all-reduce); the norm is
+ * sqrt(sumsq) * |grad_scale|, and the step uses grad * grad_scale * min(1,
+ * max_norm / (norm + 1e-6)).  The norm is written to *norm (fp32) when non-NULL
+ * (not when n is 0). */
+int mea_adamw_step_clipped(long long n, float* master, float* exp_avg, float* exp_avg_sq, const float* grad,
+                           void* param_bf16, double lr, double beta1, double beta2, double eps, double weight_decay,
+                           float grad_scale, int step, const double* sumsq, double max_norm, float* norm, void* stream);
+
+/* ---------------------------------------------------------------- gradient norm
+ * The global norm of a list of gradients and their clipping by it
+ * (torch.nn.utils.clip_grad_norm_'s rule; no counterpart in the reference).
+ * grads, n, dtypes: host arrays of `count` device pointers, element counts and
+ * MEA_BF16 / MEA_FP16 / MEA_FP32 codes; the elements of each tensor are
+ * contiguous, at any alignment of their type.  kind MEA_NORM_2: sqrt of the sum
+ * of squares (summed in fp64, also where an fp32 square would overflow);
+ * MEA_NORM_INF: the largest magnitude.  Nothing is copied to the device or back:
+ * a captured call is replayed on the same pointers. */
+enum { MEA_NORM_2 = 0, MEA_NORM_INF = 1 };
+/* Bytes of workspace for either call (8-byte aligned). */
+size_t mea_grad_norm_workspace_size(int count);
+/* *norm (fp32) and *sumsq (fp64: the sum of squares, or the largest magnitude); either may be NULL. */
+int mea_grad_norm(int count, const void* const* grads, const long long* n, const int* dtypes, int kind, float* norm,
+                  double* sumsq, void* workspace, size_t workspace_bytes, void* stream);
+/* *norm as above, and every gradient times min(1, max_norm / (norm + 1e-6)) in
+ * place (fp32 product, rounded to the gradient's type once).  No two of the
+ * tensors may overlap. */
+int mea_clip_grad_norm(int count, void* const* grads, const long long* n, const int* dtypes, int kind, double max_norm,
+                       float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- layer norm
+ * y = (x - mean) rstd w + b over the last of [rows, C] (no counterpart in the
+ * reference, whose norm has neither mean nor weight).  dtype of x, y and their
+ * gradients: MEA_BF16, MEA_FP16 or MEA_FP32; wdtype of w, b and theirs: the same
+ * or MEA_FP32.  w, b may be NULL (one, zero).  Sums are fp32.  Any C; tensors
+ * aligned to their elements (16-byte alignment and a C of whole 16-byte vectors
+ * take wider loads). */
+int mea_layernorm_forward(long long rows, int C, float eps, int dtype, int wdtype, const void* x, const void* w,
+                          const void* b, void* y, float* mean, float* rstd, void* stream);
+/* Bytes of workspace of the backward when dw or db is wanted (16-byte aligned). */
+size_t mea_layernorm_workspace_size(long long rows, int C);
+/* dx [rows, C], dw and db [C] (each may be NULL) from dy and the forward's x,
+ * mean and rstd.  dw and db are summed in a fixed order. */
+int mea_layernorm_backward(long long rows, int C, int dtype, int wdtype, const void* dy, const void* x, const void* w,
+                           const float* mean, const float* rstd, void* dx, void* dw, void* db, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- profiling
  * No counterpart in the reference (it has no timing hooks).  When enabled,
  * mea_block_forward / mea_block_backward record CUDA events on the caller's

@@ -76,6 +76,13 @@ SIGNATURES = {
     "mea_packed_plan_size": (_S, [_PD]),
     "mea_packed_attention_forward": (_I, [_PD, _P, _P, _P, _P, _P, _P, _P, _S, _P, _P]),
     "mea_packed_attention_backward": (_I, [_PD, _P, _P, _P, _P, _P, _LL, _LL, _P, _P, _S, _P, _P, _P, _P, _P, _P]),
+    "mea_layernorm_forward": (_I, [_LL, _I, _F, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "mea_layernorm_workspace_size": (_S, [_LL, _I]),
+    "mea_layernorm_backward": (_I, [_LL, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "mea_grad_norm_workspace_size": (_S, [_I]),
+    "mea_grad_norm": (_I, [_I, _P, _P, _P, _I, _P, _P, _P, _S, _P]),
+    "mea_clip_grad_norm": (_I, [_I, _P, _P, _P, _I, _DB, _P, _P, _S, _P]),
+    "mea_adamw_step_clipped": (_I, [_LL, _P, _P, _P, _P, _P, _DB, _DB, _DB, _DB, _DB, _F, _I, _P, _DB, _P, _P]),
     "mea_adamw_step": (_I, [_LL, _P, _P, _P, _P, _P, _DB, _DB, _DB, _DB, _DB, _F, _I, _P]),
     "mea_selftest_wait": (_I, [_P, ctypes.c_ulonglong, _I, _P]),
     "mea_profile_enable": (_I, [_I]),

@@ -22,7 +22,7 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libmea.so")
 
 SOURCES = ["api.cu", "gemm.cu", "attn_fwd.cu", "attn_bwd.cu", "elementwise.cu", "noalloc.cu", "optim.cu", "selftest.cu", "tma.cpp",
-           "attn_packed_plan.cu", "attn_packed_fwd.cu", "attn_packed_bwd.cu"]
+           "attn_packed_plan.cu", "attn_packed_fwd.cu", "attn_packed_bwd.cu", "layernorm.cu", "gradnorm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I" + INCLUDE, "-I" + CSRC]

@@ -1,0 +1,106 @@
+"""The global norm of a list of gradients, and clipping by it: ``grad_norm`` and
+``clip_grad_norm_`` (``mea_grad_norm``, ``mea_clip_grad_norm``).
+
+For parameters that ``ShardedAdamW`` manages, whose gradients never appear in
+``.grad``, give the optimizer ``max_grad_norm`` instead.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Iterable
+
+import torch
+
+from . import _lib
+
+_KINDS = {2.0: 0, float("inf"): 1}
+
+
+def _kind(norm_type) -> int:
+    kind = _KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    return kind
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    if t.dtype not in _lib.DTYPE_CODES or t.layout != torch.strided:
+        raise TypeError(f"gradients must be dense bf16, fp16 or fp32 tensors, got {t.dtype} ({t.layout})")
+    return t.contiguous()  # t itself where it already is
+
+
+def _arrays(tensors):
+    """(count, pointers, element counts, type codes) for the C call; every tensor contiguous, on one device."""
+    device, seen = tensors[0].device, set()
+    _lib.require_device(device)
+    ptrs, ns, codes = [], [], []
+    for t in tensors:
+        if t.device != device:
+            raise ValueError("all gradients must be on the same device")
+        p, n = t.data_ptr(), t.numel()
+        if n:
+            if p in seen:
+                raise ValueError("a gradient appears twice")
+            seen.add(p)
+        ptrs.append(p)
+        ns.append(n)
+        codes.append(_lib.DTYPE_CODES[t.dtype])
+    k = len(tensors)
+    return k, (ctypes.c_void_p * k)(*ptrs), (ctypes.c_longlong * k)(*ns), (ctypes.c_int * k)(*codes)
+
+
+def _workspace(k, device):
+    nbytes = _lib.lib().mea_grad_norm_workspace_size(k)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all elements of ``tensors`` as one vector: a 0-dim fp32 tensor on their device (no copy to the
+    host).  ``norm_type`` 2 or inf.  An empty list has norm 0 (on the CPU)."""
+    kind = _kind(norm_type)
+    tensors = [_dense(t) for t in tensors]
+    if not tensors:
+        return torch.tensor(0.0)
+    k, ptrs, ns, codes = _arrays(tensors)
+    device = tensors[0].device
+    out = torch.empty((), dtype=torch.float32, device=device)
+    with _lib.on_device(device):
+        ws, nbytes = _workspace(k, device)
+        _lib.check(_lib.lib().mea_grad_norm(k, ptrs, ns, codes, kind, out.data_ptr(), None, ws.data_ptr(), nbytes,
+                                            _lib.stream_ptr(device)))
+    return out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Multiplies the gradients of ``parameters`` (a tensor or an iterable; those without ``.grad`` are passed over) in
+    place by min(1, max_norm / (norm + 1e-6)), where norm is the global norm of them all, and returns that norm: a 0-dim
+    fp32 tensor on their device.  torch.nn.utils.clip_grad_norm_'s rule, in two kernels over the whole list: one reads
+    every gradient, the other scales, and does nothing where the norm is within max_norm.  The factor is applied in fp32
+    and rounded to the gradient's type once.  ``error_if_nonfinite`` waits for the norm and raises before anything is
+    scaled."""
+    kind = _kind(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    work = [_dense(g) for g in grads]
+    k, ptrs, ns, codes = _arrays(work)
+    device = work[0].device
+    if error_if_nonfinite:
+        norm = grad_norm(work, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total norm of order {norm_type} of the gradients is non-finite, so they cannot be clipped")
+    out = torch.empty((), dtype=torch.float32, device=device)
+    with _lib.on_device(device):
+        ws, nbytes = _workspace(k, device)
+        _lib.check(_lib.lib().mea_clip_grad_norm(k, ptrs, ns, codes, kind, max_norm, out.data_ptr(), ws.data_ptr(), nbytes,
+                                                 _lib.stream_ptr(device)))
+        for g, w in zip(grads, work):
+            if g is not w:
+                g.copy_(w)
+    return out

@@ -749,6 +749,14 @@ int mea_adamw_step(long long n, float* master, float* exp_avg, float* exp_avg_sq
                    step, static_cast<cudaStream_t>(stream));
 }
 
+int mea_adamw_step_clipped(long long n, float* master, float* exp_avg, float* exp_avg_sq, const float* grad,
+                           void* param_bf16, double lr, double beta1, double beta2, double eps, double weight_decay,
+                           float grad_scale, int step, const double* sumsq, double max_norm, float* norm, void* stream) {
+  if (!sumsq) return set_error(MEA_ERR_INVALID_ARGUMENT, "adamw: sumsq is NULL");
+  return run_adamw(n, master, exp_avg, exp_avg_sq, grad, param_bf16, lr, beta1, beta2, eps, weight_decay, grad_scale,
+                   step, static_cast<cudaStream_t>(stream), sumsq, max_norm, norm);
+}
+
 int mea_profile_enable(int on) {
   std::lock_guard<std::mutex> lock(g_prof.mu);
   for (auto& r : g_prof.recs) {

@@ -103,6 +103,6 @@ int run_rope_bound(int T, int HD, const void* f1, const void* f2, long long ldf,
 // ---- optimizer (optim.cu) ----
 int run_adamw(long long n, float* master, float* exp_avg, float* exp_avg_sq, const float* grad, void* param,
               double lr, double beta1, double beta2, double eps, double weight_decay, float grad_scale, int step,
-              cudaStream_t st);
+              cudaStream_t st, const double* sumsq = nullptr, double max_norm = 0.0, float* norm = nullptr);
 
 }  // namespace mea

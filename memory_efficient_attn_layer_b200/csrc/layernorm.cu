@@ -1,0 +1,598 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   y = (x - mean) rstd w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   g = dy w,  xhat = (x - mean) rstd
+//   dx = rstd (g - mean(g) - xhat mean(g xhat)),  dw = sum_rows dy xhat,  db = sum_rows dy
+//
+// Both directions are bound by HBM: the forward reads x and writes y, the
+// backward reads x and dy and writes dx.  A row stays in the registers of the
+// TPR threads that share it, so it is read once although the variance is taken
+// about the mean (a second sum, not a difference of large ones).  In the
+// backward each thread keeps its own columns for every row that its block takes,
+// so dw and db grow in registers; each block writes one fp32 partial row and a
+// second kernel adds those in a fixed order.  All sums are fp32.
+//
+// Rows too long for that (above 16384 elements) take kernels that walk the row
+// several times, and a column-wise pass for dw and db.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace mea {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// VEC values at p (VEC = 1, or 16 bytes of T; weights of another type take two 16-byte loads).
+template <int VEC, class T>
+__device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    f[0] = to_f(*p);
+  } else {
+    constexpr int PER = 16 / sizeof(T);
+    static_assert(VEC % PER == 0, "");
+#pragma unroll
+    for (int i = 0; i < VEC / PER; ++i) {
+      const uint4 r = reinterpret_cast<const uint4*>(p)[i];
+      T t[PER];
+      *reinterpret_cast<uint4*>(t) = r;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) f[i * PER + e] = to_f(t[e]);
+    }
+  }
+}
+template <int VEC, class T>
+__device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = from_f<T>(f[0]);
+  } else {
+    T t[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) t[e] = from_f<T>(f[e]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(t);
+  }
+}
+
+// Sums K values over each group of TPR threads; every thread gets the sums.
+// One block barrier: `red` holds two sets, used in turn.
+template <int TPR, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float* red, int& turn) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
+  if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    const int warp = threadIdx.x >> 5, all = blockDim.x >> 5;
+    float* r = red + turn * all * K;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) r[warp * K + k] = v[k];
+    __syncthreads();
+    const float* first = r + (warp / WARPS) * WARPS * K;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += first[w * K + k];
+  }
+}
+
+template <int TPR>
+constexpr int ln_threads() {
+  return TPR > 256 ? TPR : 256;
+}
+
+template <class T, class W, int VEC, int TPR, int V>
+__global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_fwd_kernel(long long rows, int C, float eps,
+                                                                         const T* __restrict__ x,
+                                                                         const W* __restrict__ w,
+                                                                         const W* __restrict__ b, T* __restrict__ y,
+                                                                         float* __restrict__ mean_out,
+                                                                         float* __restrict__ rstd_out) {
+  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR;
+  __shared__ float red[2 * THREADS / 32];
+  int turn = 0;
+  const int g = threadIdx.x / TPR, lane = threadIdx.x % TPR;
+  const float inv_c = 1.0f / float(C);
+  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < rows; row0 += (long long)gridDim.x * GROUPS) {
+    const long long row = row0 + g;
+    const bool live = row < rows;
+    const T* xr = x + row * C;
+    float f[V][VEC];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * TPR + lane) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[v][e] = 0.f;
+      if (live && c < C) load_vec<VEC>(xr + c, f[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[0] += f[v][e];
+    group_sum<TPR>(s, red, turn);
+    const float mean = s[0] * inv_c;
+    s[0] = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if ((v * TPR + lane) * VEC < C)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          f[v][e] -= mean;
+          s[0] += f[v][e] * f[v][e];
+        }
+    group_sum<TPR>(s, red, turn);
+    const float rstd = 1.0f / sqrtf(s[0] * inv_c + eps);
+    if (!live) continue;  // the loop's trip count is the block's, not the group's
+    if (lane == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    T* yr = y + row * C;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * TPR + lane) * VEC;
+      if (c >= C) continue;
+      float ww[VEC], bb[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        ww[e] = 1.f;
+        bb[e] = 0.f;
+      }
+      if (w) load_vec<VEC>(w + c, ww);
+      if (b) load_vec<VEC>(b + c, bb);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[v][e] = f[v][e] * rstd * ww[e] + bb[e];
+      store_vec<VEC>(yr + c, f[v]);
+    }
+  }
+}
+
+// R rows per group and round; block i takes every gridDim.x-th round.  Partial
+// sums of the block's rows: part[(2 i) C ..] for dw, part[(2 i + 1) C ..] for db.
+template <class T, class W, int VEC, int TPR, int V, int R>
+__global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_bwd_kernel(long long rows, int C,
+                                                                         const T* __restrict__ dy,
+                                                                         const T* __restrict__ x,
+                                                                         const W* __restrict__ w,
+                                                                         const float* __restrict__ mean_in,
+                                                                         const float* __restrict__ rstd_in,
+                                                                         T* __restrict__ dx, float* __restrict__ part) {
+  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR;
+  __shared__ float red[2 * 2 * R * THREADS / 32];
+  extern __shared__ float cols[];  // [2][C], only with several groups
+  pdl_launch();
+  int turn = 0;
+  const int g = threadIdx.x / TPR, lane = threadIdx.x % TPR;
+  const float inv_c = 1.0f / float(C);
+  float ww[V][VEC], dw[V][VEC], db[V][VEC];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (v * TPR + lane) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      ww[v][e] = 1.f;
+      dw[v][e] = db[v][e] = 0.f;
+    }
+    if (w && c < C) load_vec<VEC>(w + c, ww[v]);
+  }
+  for (long long row0 = (long long)blockIdx.x * GROUPS * R; row0 < rows; row0 += (long long)gridDim.x * GROUPS * R) {
+    float xf[R][V][VEC], df[R][V][VEC], rstd[R], sums[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = row0 + g * R + r;
+      const bool live = row < rows;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = (v * TPR + lane) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) xf[r][v][e] = df[r][v][e] = 0.f;
+        if (live && c < C) {
+          load_vec<VEC>(x + row * C + c, xf[r][v]);
+          load_vec<VEC>(dy + row * C + c, df[r][v]);
+        }
+      }
+      rstd[r] = live ? rstd_in[row] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = row0 + g * R + r;
+      const float mean = row < rows ? mean_in[row] : 0.f;
+      sums[2 * r] = sums[2 * r + 1] = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if ((v * TPR + lane) * VEC >= C) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          xf[r][v][e] = (xf[r][v][e] - mean) * rstd[r];
+          const float gg = df[r][v][e] * ww[v][e];
+          sums[2 * r] += gg;
+          sums[2 * r + 1] += gg * xf[r][v][e];
+          dw[v][e] += df[r][v][e] * xf[r][v][e];
+          db[v][e] += df[r][v][e];
+        }
+      }
+    }
+    group_sum<TPR>(sums, red, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = row0 + g * R + r;
+      if (row >= rows) continue;
+      const float m1 = sums[2 * r] * inv_c, m2 = sums[2 * r + 1] * inv_c;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = (v * TPR + lane) * VEC;
+        if (c >= C) continue;
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = rstd[r] * (df[r][v][e] * ww[v][e] - m1 - xf[r][v][e] * m2);
+        store_vec<VEC>(dx + row * C + c, o);
+      }
+    }
+  }
+  if (!part) return;
+  float* out = part + (long long)blockIdx.x * 2 * C;
+  if (GROUPS > 1) {  // the groups' sums, added in their order
+    for (int k = 0; k < GROUPS; ++k) {
+      if (g == k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int c = (v * TPR + lane) * VEC;
+          if (c >= C) continue;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            cols[c + e] = (k ? cols[c + e] : 0.f) + dw[v][e];
+            cols[C + c + e] = (k ? cols[C + c + e] : 0.f) + db[v][e];
+          }
+        }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 2 * C; i += THREADS) out[i] = cols[i];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * TPR + lane) * VEC;
+      if (c >= C) continue;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        out[c + e] = dw[v][e];
+        out[C + c + e] = db[v][e];
+      }
+    }
+  }
+}
+
+// dw (blockIdx.y = 0) and db (1): column sums of `n` partial rows, 32 columns a
+// block, 32 slices of rows added in order, then the slices in order.
+template <class W>
+__global__ void __launch_bounds__(1024) layernorm_cols_kernel(int n, int C, const float* __restrict__ part,
+                                                              W* __restrict__ dw, W* __restrict__ db) {
+  __shared__ float s[32][33];
+  pdl_wait();
+  W* out = blockIdx.y ? db : dw;
+  if (!out) return;
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float a = 0.f;
+  if (c < C)
+    for (int i = threadIdx.y; i < n; i += 32) a += part[((long long)2 * i + blockIdx.y) * C + c];
+  s[threadIdx.y][threadIdx.x] = a;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < C) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += s[i][threadIdx.x];
+    out[c] = from_f<W>(t);
+  }
+}
+
+// ---- rows longer than the register path takes: one block per row, the row walked several times ----
+__device__ __forceinline__ float block_sum(float v, float* red, int& turn) {
+  float a[1] = {v};
+  group_sum<1024>(a, red, turn);
+  return a[0];
+}
+template <class T, class W>
+__global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(long long rows, int C, float eps,
+                                                                  const T* __restrict__ x, const W* __restrict__ w,
+                                                                  const W* __restrict__ b, T* __restrict__ y,
+                                                                  float* __restrict__ mean_out,
+                                                                  float* __restrict__ rstd_out) {
+  __shared__ float red[64];
+  int turn = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * C;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < C; c += 1024) s += to_f(xr[c]);
+    const float mean = block_sum(s, red, turn) / float(C);
+    s = 0.f;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float d = to_f(xr[c]) - mean;
+      s += d * d;
+    }
+    const float rstd = 1.0f / sqrtf(block_sum(s, red, turn) / float(C) + eps);
+    if (threadIdx.x == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+    for (int c = threadIdx.x; c < C; c += 1024)
+      y[row * C + c] = from_f<T>((to_f(xr[c]) - mean) * rstd * (w ? to_f(w[c]) : 1.f) + (b ? to_f(b[c]) : 0.f));
+  }
+}
+template <class T, class W>
+__global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(long long rows, int C, const T* __restrict__ dy,
+                                                                  const T* __restrict__ x, const W* __restrict__ w,
+                                                                  const float* __restrict__ mean_in,
+                                                                  const float* __restrict__ rstd_in,
+                                                                  T* __restrict__ dx) {
+  __shared__ float red[64];
+  int turn = 0;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T *xr = x + row * C, *dr = dy + row * C;
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float gg = to_f(dr[c]) * (w ? to_f(w[c]) : 1.f);
+      s1 += gg;
+      s2 += gg * ((to_f(xr[c]) - mean) * rstd);
+    }
+    const float m1 = block_sum(s1, red, turn) / float(C), m2 = block_sum(s2, red, turn) / float(C);
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float gg = to_f(dr[c]) * (w ? to_f(w[c]) : 1.f);
+      dx[row * C + c] = from_f<T>(rstd * (gg - m1 - (to_f(xr[c]) - mean) * rstd * m2));
+    }
+  }
+}
+// Partial column sums: block (i, j) adds rows i, i + gridDim.y, ... of columns [256 j, 256 j + 256).
+template <class T>
+__global__ void __launch_bounds__(256) layernorm_part_long_kernel(long long rows, int C, const T* __restrict__ dy,
+                                                                  const T* __restrict__ x,
+                                                                  const float* __restrict__ mean_in,
+                                                                  const float* __restrict__ rstd_in,
+                                                                  float* __restrict__ part) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= C) return;
+  float dw = 0.f, db = 0.f;
+  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float d = to_f(dy[row * C + c]);
+    dw += d * ((to_f(x[row * C + c]) - mean_in[row]) * rstd_in[row]);
+    db += d;
+  }
+  part[((long long)2 * blockIdx.y) * C + c] = dw;
+  part[((long long)2 * blockIdx.y + 1) * C + c] = db;
+}
+
+// ---------------------------------------------------------------- host side
+// Register path: TPR threads with V vectors of VEC elements each hold a row.
+struct LnShape {
+  int vec, tpr, v;  // v = 0: the long-row kernels
+};
+static LnShape ln_shape(int C, int elem, bool aligned) {
+  LnShape s;
+  s.vec = aligned && C % (16 / elem) == 0 ? 16 / elem : 1;
+  const int units = (C + s.vec - 1) / s.vec;
+  s.tpr = 32;
+  const int most = s.vec == 1 ? 8 : 1;  // vectors (or single elements) a thread takes before the next doubling of TPR
+  while (s.tpr < 512 && s.tpr * most < units) s.tpr *= 2;
+  s.v = 1;
+  while (s.tpr * s.v < units) s.v *= 2;
+  if (s.vec == 1 && s.v < 8) s.v = 8;
+  if (s.vec * s.v > 32) s.v = 0;
+  return s;
+}
+constexpr int LN_LONG_PARTS = 64;
+
+static int ln_bwd_blocks(long long rows, const LnShape& s, int rows_per_round) {
+  const int threads = s.tpr > 256 ? s.tpr : 256, groups = threads / s.tpr;
+  const long long rounds = (rows + (long long)groups * rows_per_round - 1) / ((long long)groups * rows_per_round);
+  return int(std::min<long long>(rounds, (long long)num_sms() * (threads > 256 ? 1 : 2)));
+}
+// Rows in flight per group: as many as keep the row registers (x and dy) near 64.
+template <int VEC, int V>
+constexpr int ln_rows() {
+  return VEC * V >= 32 ? 1 : VEC * V >= 16 ? 2 : 4;
+}
+
+template <class T, class W, int VEC, int TPR, int V>
+static void ln_fwd(long long rows, int C, float eps, const void* x, const void* w, const void* b, void* y, float* mean,
+                   float* rstd, cudaStream_t st) {
+  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR;
+  const long long rounds = (rows + GROUPS - 1) / GROUPS;
+  const int grid = int(std::min<long long>(rounds, (long long)num_sms() * (2048 / THREADS)));
+  layernorm_fwd_kernel<T, W, VEC, TPR, V><<<grid, THREADS, 0, st>>>(
+      rows, C, eps, static_cast<const T*>(x), static_cast<const W*>(w), static_cast<const W*>(b), static_cast<T*>(y), mean,
+      rstd);
+}
+template <class T, class W, int VEC, int TPR, int V>
+static void ln_bwd(long long rows, int C, const void* dy, const void* x, const void* w, const float* mean,
+                   const float* rstd, void* dx, float* part, int grid, cudaStream_t st) {
+  constexpr int THREADS = ln_threads<TPR>();
+  const size_t smem = THREADS > TPR && part ? size_t(2) * C * sizeof(float) : 0;
+  layernorm_bwd_kernel<T, W, VEC, TPR, V, ln_rows<VEC, V>()><<<grid, THREADS, smem, st>>>(
+      rows, C, static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const W*>(w), mean, rstd,
+      static_cast<T*>(dx), part);
+}
+
+// Calls f.template run<VEC, TPR, V>() for the shape: with 16-byte vectors TPR
+// grows first (V = 1 below TPR = 512); with single elements V = 8 below that.
+template <int FULL, class F>
+static void ln_dispatch(const LnShape& s, F&& f) {
+  auto tpr = [&](auto vec, auto v) {
+    switch (s.tpr) {
+      case 32: f(vec, std::integral_constant<int, 32>(), v); break;
+      case 64: f(vec, std::integral_constant<int, 64>(), v); break;
+      case 128: f(vec, std::integral_constant<int, 128>(), v); break;
+      case 256: f(vec, std::integral_constant<int, 256>(), v); break;
+      default: f(vec, std::integral_constant<int, 512>(), v); break;
+    }
+  };
+  using std::integral_constant;
+  if (s.vec == 1) {
+    integral_constant<int, 1> one;
+    if (s.v == 8) return tpr(one, integral_constant<int, 8>());
+    integral_constant<int, 512> all;
+    return s.v == 16 ? f(one, all, integral_constant<int, 16>()) : f(one, all, integral_constant<int, 32>());
+  }
+  integral_constant<int, FULL> vec;
+  if (s.v == 1) return tpr(vec, integral_constant<int, 1>());
+  integral_constant<int, 512> all;
+  if (s.v == 2) return f(vec, all, integral_constant<int, 2>());
+  if (s.v == 4) return f(vec, all, integral_constant<int, 4>());
+  if constexpr (FULL == 4) f(vec, all, integral_constant<int, 8>());
+}
+
+template <class T, class W>
+static int layernorm_fwd(long long rows, int C, float eps, const void* x, const void* w, const void* b, void* y,
+                         float* mean, float* rstd, const LnShape& s, cudaStream_t st) {
+  if (s.v == 0) {
+    const int grid = int(std::min<long long>(rows, (long long)num_sms() * 2));
+    layernorm_fwd_long_kernel<T, W><<<grid, 1024, 0, st>>>(rows, C, eps, static_cast<const T*>(x),
+                                                           static_cast<const W*>(w), static_cast<const W*>(b),
+                                                           static_cast<T*>(y), mean, rstd);
+  } else {
+    ln_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
+      ln_fwd<T, W, vec(), tpr(), v()>(rows, C, eps, x, w, b, y, mean, rstd, st);
+    });
+  }
+  return check_launch("layernorm_fwd_kernel");
+}
+
+static int ln_rows_of(const LnShape& s) { return s.vec * s.v >= 32 ? 1 : s.vec * s.v >= 16 ? 2 : 4; }
+
+template <class T, class W>
+static int layernorm_bwd(long long rows, int C, const void* dy, const void* x, const void* w, const float* mean,
+                         const float* rstd, void* dx, void* dw, void* db, float* part, const LnShape& s,
+                         cudaStream_t st) {
+  int parts = 0;
+  if (rows > 0) {
+    if (s.v == 0) {
+      const int grid = int(std::min<long long>(rows, (long long)num_sms() * 2));
+      layernorm_bwd_long_kernel<T, W><<<grid, 1024, 0, st>>>(rows, C, static_cast<const T*>(dy), static_cast<const T*>(x),
+                                                             static_cast<const W*>(w), mean, rstd, static_cast<T*>(dx));
+      if (part) {
+        parts = int(std::min<long long>(rows, LN_LONG_PARTS));
+        layernorm_part_long_kernel<T><<<dim3(unsigned((C + 255) / 256), unsigned(parts)), 256, 0, st>>>(
+            rows, C, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, part);
+      }
+    } else {
+      parts = ln_bwd_blocks(rows, s, ln_rows_of(s));
+      ln_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
+        ln_bwd<T, W, vec(), tpr(), v()>(rows, C, dy, x, w, mean, rstd, dx, part, parts, st);
+      });
+    }
+    const int rc = check_launch("layernorm_bwd_kernel");
+    if (rc != MEA_OK) return rc;
+  }
+  if (!part) return MEA_OK;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned((C + 31) / 32), 2);
+  cfg.blockDim = dim3(32, 32);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, layernorm_cols_kernel<W>, parts, C, static_cast<const float*>(part), static_cast<W*>(dw),
+                     static_cast<W*>(db));
+  return check_launch("layernorm_cols_kernel");
+}
+
+static int ln_check(long long rows, int C, int dtype, int wdtype) {
+  if (rows < 0 || C <= 0)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "layer norm: rows=%lld must be >= 0 and C=%d positive", rows, C);
+  if (dtype != MEA_BF16 && dtype != MEA_FP16 && dtype != MEA_FP32)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "layer norm: dtype %d is none of MEA_BF16, MEA_FP16, MEA_FP32", dtype);
+  if (wdtype != dtype && wdtype != MEA_FP32)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "layer norm: the weight's dtype %d is neither x's (%d) nor MEA_FP32", wdtype,
+                     dtype);
+  return MEA_OK;
+}
+static int ln_align(std::initializer_list<const void*> ps, int elem) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % elem)
+      return set_error(MEA_ERR_ALIGNMENT, "layer norm: a tensor is not aligned to its %d-byte elements", elem);
+  return MEA_OK;
+}
+static bool ln_vector(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+  return true;
+}
+
+}  // namespace mea
+
+extern "C" size_t mea_layernorm_workspace_size(long long rows, int C) {
+  if (rows < 0 || C <= 0) return 0;
+  // dw and db partials of at most two blocks an SM, on the largest part there is
+  return size_t(2) * size_t(C) * sizeof(float) * 2 * 160;
+}
+
+extern "C" int mea_layernorm_forward(long long rows, int C, float eps, int dtype, int wdtype, const void* x, const void* w,
+                                     const void* b, void* y, float* mean, float* rstd, void* stream) {
+  using namespace mea;
+  int rc = ln_check(rows, C, dtype, wdtype);
+  if (rc != MEA_OK) return rc;
+  if (!(eps >= 0.f) || !(eps < 3.0e38f)) return set_error(MEA_ERR_INVALID_ARGUMENT, "layer norm: eps=%g must be >= 0", eps);
+  if (rows == 0) return MEA_OK;
+  if (!x || !y || !mean || !rstd) return set_error(MEA_ERR_INVALID_ARGUMENT, "layer norm: x, y, mean and rstd must be non-NULL");
+  const int elem = dtype == MEA_FP32 ? 4 : 2;
+  if ((rc = ln_align({x, y}, elem)) != MEA_OK || (rc = ln_align({mean, rstd}, 4)) != MEA_OK ||
+      (rc = ln_align({w, b}, wdtype == MEA_FP32 ? 4 : 2)) != MEA_OK)
+    return rc;
+  auto st = static_cast<cudaStream_t>(stream);
+  const LnShape s = ln_shape(C, elem, ln_vector({x, y, w, b}));
+  if (dtype == MEA_FP32) return layernorm_fwd<float, float>(rows, C, eps, x, w, b, y, mean, rstd, s, st);
+  if (dtype == MEA_BF16)
+    return wdtype == MEA_FP32 ? layernorm_fwd<__nv_bfloat16, float>(rows, C, eps, x, w, b, y, mean, rstd, s, st)
+                              : layernorm_fwd<__nv_bfloat16, __nv_bfloat16>(rows, C, eps, x, w, b, y, mean, rstd, s, st);
+  return wdtype == MEA_FP32 ? layernorm_fwd<__half, float>(rows, C, eps, x, w, b, y, mean, rstd, s, st)
+                            : layernorm_fwd<__half, __half>(rows, C, eps, x, w, b, y, mean, rstd, s, st);
+}
+
+extern "C" int mea_layernorm_backward(long long rows, int C, int dtype, int wdtype, const void* dy, const void* x,
+                                      const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mea;
+  int rc = ln_check(rows, C, dtype, wdtype);
+  if (rc != MEA_OK) return rc;
+  const bool sums = dw || db;
+  if (rows == 0 && !sums) return MEA_OK;
+  if (rows > 0 && (!dy || !x || !mean || !rstd || !dx))
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "layer norm backward: dy, x, mean, rstd and dx must be non-NULL");
+  const int elem = dtype == MEA_FP32 ? 4 : 2;
+  if ((rc = ln_align({dy, x, dx}, elem)) != MEA_OK || (rc = ln_align({mean, rstd}, 4)) != MEA_OK ||
+      (rc = ln_align({w, dw, db}, wdtype == MEA_FP32 ? 4 : 2)) != MEA_OK)
+    return rc;
+  if (sums && (!workspace || reinterpret_cast<uintptr_t>(workspace) & 15))
+    return set_error(MEA_ERR_ALIGNMENT, "layer norm backward: the workspace must be non-NULL and 16-byte aligned");
+  if (sums && workspace_bytes < mea_layernorm_workspace_size(rows, C))
+    return set_error(MEA_ERR_WORKSPACE, "layer norm backward: the workspace has %zu bytes, needs %zu", workspace_bytes,
+                     mea_layernorm_workspace_size(rows, C));
+  auto st = static_cast<cudaStream_t>(stream);
+  float* part = sums ? static_cast<float*>(workspace) : nullptr;
+  const LnShape s = ln_shape(C, elem, ln_vector({dy, x, dx, w}));
+  if (dtype == MEA_FP32) return layernorm_bwd<float, float>(rows, C, dy, x, w, mean, rstd, dx, dw, db, part, s, st);
+  if (dtype == MEA_BF16)
+    return wdtype == MEA_FP32
+               ? layernorm_bwd<__nv_bfloat16, float>(rows, C, dy, x, w, mean, rstd, dx, dw, db, part, s, st)
+               : layernorm_bwd<__nv_bfloat16, __nv_bfloat16>(rows, C, dy, x, w, mean, rstd, dx, dw, db, part, s, st);
+  return wdtype == MEA_FP32 ? layernorm_bwd<__half, float>(rows, C, dy, x, w, mean, rstd, dx, dw, db, part, s, st)
+                            : layernorm_bwd<__half, __half>(rows, C, dy, x, w, mean, rstd, dx, dw, db, part, s, st);
+}

@@ -11,12 +11,17 @@
 // with g = grad * grad_scale (1/world for the mean over data-parallel ranks).
 // One HBM pass: 16 bytes read and 12 written per element of fp32 state, plus
 // the 2-byte bf16 copy of the new weight.
+//
+// Clipping by the global norm costs no pass of its own here: given the sum of
+// squares of every gradient (a device scalar), the factor min(1, max_norm /
+// (norm + 1e-6)) multiplies grad_scale.
 #include <cuda_bf16.h>
 
 #include <algorithm>
 #include <cmath>
 
 #include "launch.h"
+#include "ptx.cuh"
 
 namespace mea {
 
@@ -44,7 +49,19 @@ __device__ __forceinline__ float adamw_one(float& w, float& m, float& v, float g
 // Grid-stride over float4 groups; the last n % 4 elements go one per thread.
 __global__ void __launch_bounds__(256) adamw_kernel(long long n, float* __restrict__ master, float* __restrict__ exp_avg,
                                                     float* __restrict__ exp_avg_sq, const float* __restrict__ grad,
-                                                    __nv_bfloat16* __restrict__ param, AdamWConsts c) {
+                                                    __nv_bfloat16* __restrict__ param, AdamWConsts c,
+                                                    const double* __restrict__ sumsq, double max_norm,
+                                                    float* __restrict__ norm_out) {
+  if (sumsq) {
+    __shared__ float factor;
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(*sumsq) * fabs(double(c.grad_scale));  // of the scaled gradient
+      factor = clip_factor(norm, max_norm);
+      if (blockIdx.x == 0 && norm_out) *norm_out = float(norm);
+    }
+    __syncthreads();
+    c.grad_scale *= factor;
+  }
   const long long n4 = n >> 2;
   const long long stride = (long long)gridDim.x * blockDim.x;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += stride) {
@@ -81,7 +98,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(long long n, float* __restri
 
 int run_adamw(long long n, float* master, float* exp_avg, float* exp_avg_sq, const float* grad, void* param,
               double lr, double beta1, double beta2, double eps, double weight_decay, float grad_scale, int step,
-              cudaStream_t st) {
+              cudaStream_t st, const double* sumsq, double max_norm, float* norm) {
   if (n < 0) return set_error(MEA_ERR_INVALID_ARGUMENT, "adamw: n=%lld must be >= 0", n);
   if (n == 0) return MEA_OK;
   if (!master || !exp_avg || !exp_avg_sq || !grad)
@@ -96,6 +113,10 @@ int run_adamw(long long n, float* master, float* exp_avg, float* exp_avg_sq, con
       return set_error(MEA_ERR_ALIGNMENT, "adamw: fp32 buffers must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(param) % 8)
     return set_error(MEA_ERR_ALIGNMENT, "adamw: the bf16 weights must be 8-byte aligned");
+  if (sumsq && !(max_norm >= 0.0))
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "adamw: max_norm=%g must be >= 0", max_norm);
+  if (reinterpret_cast<uintptr_t>(sumsq) % 8 || reinterpret_cast<uintptr_t>(norm) % 4)
+    return set_error(MEA_ERR_ALIGNMENT, "adamw: sumsq must be 8-byte, norm 4-byte aligned");
   // Scalar schedule in double, rounded to fp32 once per constant (the values
   // torch.optim.AdamW's per-tensor arithmetic receives from Python floats).
   const double bc1 = 1.0 - std::pow(beta1, double(step));
@@ -114,7 +135,7 @@ int run_adamw(long long n, float* master, float* exp_avg, float* exp_avg_sq, con
   const long long cap = (long long)num_sms() * 8;  // 8 resident CTAs of 256 threads per SM
   const int blocks = int(std::max<long long>(1, std::min(want, cap)));
   adamw_kernel<<<blocks, threads, 0, st>>>(n, master, exp_avg, exp_avg_sq, grad,
-                                           static_cast<__nv_bfloat16*>(param), c);
+                                           static_cast<__nv_bfloat16*>(param), c, sumsq, max_norm, norm);
   return check_launch("adamw_kernel");
 }
 

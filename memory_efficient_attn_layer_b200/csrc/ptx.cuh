@@ -521,6 +521,12 @@ __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v 
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
 __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
+// Clipping by the global norm: min(1, max_norm / (norm + 1e-6)) in fp64, rounded to fp32; NaN stays.
+__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
+  const double f = max_norm / (norm + 1e-6);
+  return f > 1.0 ? 1.0f : float(f);
+}
+
 __device__ __forceinline__ void st_global_v4(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }

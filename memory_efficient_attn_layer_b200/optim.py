@@ -26,6 +26,7 @@ is added in at ``step()``.  ``zero_grad()`` clears both.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Iterable, Optional
 
 import torch
@@ -149,6 +150,14 @@ class ShardedAdamW(torch.optim.Optimizer):
     None).  The weights must start identical on every rank; the first rank's
     are broadcast at construction.
 
+    ``max_grad_norm``: clip each step's gradient (after averaging) by its global
+    norm over all weights and ranks, times min(1, max_grad_norm / (norm + 1e-6)),
+    as ``clip_grad_norm_`` does for gradients in ``.grad``.  The factor goes into
+    the update kernel, so clipping costs one read of the shard's gradients (and
+    one all-reduce of a scalar between ranks); after ``step()`` the norm is in
+    ``grad_norm`` (0-dim fp32 tensor on the device; None before the first step
+    or without ``max_grad_norm``).
+
     Every ``step()`` updates every managed weight: a weight that received no
     gradient since ``zero_grad()`` is stepped with a zero gradient (its moments
     decay and weight decay applies), where torch.optim.AdamW would skip it.
@@ -157,7 +166,7 @@ class ShardedAdamW(torch.optim.Optimizer):
 
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, group=None, average: bool = True,
-                 fused_grads: bool = True):
+                 fused_grads: bool = True, max_grad_norm: Optional[float] = None):
         params = list(params)
         if not lr >= 0.0:
             raise ValueError(f"invalid learning rate {lr}")
@@ -167,6 +176,8 @@ class ShardedAdamW(torch.optim.Optimizer):
             raise ValueError(f"invalid betas {betas}")
         if not weight_decay >= 0.0:
             raise ValueError(f"invalid weight_decay {weight_decay}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"invalid max_grad_norm {max_grad_norm}")
         for p in params:
             if p.dtype != torch.bfloat16:
                 raise TypeError(f"ShardedAdamW updates bf16 parameters; got {p.dtype}")
@@ -186,6 +197,8 @@ class ShardedAdamW(torch.optim.Optimizer):
         self.grad_shard = L.grad32 if single else torch.empty(S, dtype=torch.float32, device=L.flat.device)
         self.param_shard = L.flat if single else torch.empty(S, dtype=torch.bfloat16, device=L.flat.device)
         self.steps = 0
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.grad_norm = None
         self._written = set()
         _dp.register_grad_sink(self)
 
@@ -224,13 +237,32 @@ class ShardedAdamW(torch.optim.Optimizer):
         scale = 1.0 / L.world if self.average else 1.0
         lib = _lib.lib()
         dev = L.flat.device
-        _lib.check(lib.mea_adamw_step(
-            L.shard, _lib.ptr(self.master), _lib.ptr(self.exp_avg), _lib.ptr(self.exp_avg_sq),
-            _lib.ptr(self.grad_shard), _lib.ptr(self.param_shard), float(g["lr"]), float(g["betas"][0]),
-            float(g["betas"][1]), float(g["eps"]), float(g["weight_decay"]), scale, self.steps,
-            _lib.stream_ptr(dev)))
+        args = (L.shard, _lib.ptr(self.master), _lib.ptr(self.exp_avg), _lib.ptr(self.exp_avg_sq),
+                _lib.ptr(self.grad_shard), _lib.ptr(self.param_shard), float(g["lr"]), float(g["betas"][0]),
+                float(g["betas"][1]), float(g["eps"]), float(g["weight_decay"]), scale, self.steps)
+        if self.max_grad_norm is None:
+            _lib.check(lib.mea_adamw_step(*args, _lib.stream_ptr(dev)))
+        else:
+            with _lib.on_device(dev):
+                sumsq = self._sum_of_squares()
+                self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
+                _lib.check(lib.mea_adamw_step_clipped(*args, sumsq.data_ptr(), self.max_grad_norm,
+                                                      self.grad_norm.data_ptr(), _lib.stream_ptr(dev)))
         L.all_gather(self.param_shard)
         return loss
+
+    def _sum_of_squares(self) -> torch.Tensor:
+        """fp64 scalar: the sum of squares of the summed gradient over every rank's shard."""
+        L, lib, dev = self.layout, _lib.lib(), self.layout.flat.device
+        nbytes = lib.mea_grad_norm_workspace_size(1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        sumsq = torch.empty((), dtype=torch.float64, device=dev)
+        _lib.check(lib.mea_grad_norm(
+            1, (ctypes.c_void_p * 1)(self.grad_shard.data_ptr()), (ctypes.c_longlong * 1)(L.shard),
+            (ctypes.c_int * 1)(_lib.MEA_FP32), 0, None, sumsq.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_ptr(dev)))
+        if L.world > 1:
+            dist.all_reduce(sumsq, group=L.group)
+        return sumsq
 
     # -- checkpoints (this rank's shard) ---------------------------------------------
     def state_dict(self) -> dict:
