@@ -10,6 +10,7 @@ import ctypes
 import os
 import re
 import threading
+import time
 
 import torch
 
@@ -162,8 +163,12 @@ class _StatusWatch:
         self.word = torch.zeros(1, dtype=torch.int32, device=device)
         self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
         self.event = None
+        self.address = self.word.data_ptr()
+        self.pending = False  # launches behind the last copy
+        self.next_note = 0.0
 
     def note(self) -> None:
+        self.pending = False
         self.host.copy_(self.word, non_blocking=True)
         if self.event is None:
             self.event = torch.cuda.Event()
@@ -231,45 +236,63 @@ def poll_status(device: torch.device) -> None:
         raise _timeout_error(v, "in an earlier call")
 
 
-def status_word(device: torch.device) -> int:
-    """Address of the device's status word.  It is allocated by the first call on
-    the device, which must not be a captured one: the word would belong to that
-    graph's memory."""
-    if _device_index(device) not in _watch and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the first call on a device must come before a stream capture (it allocates the status word)")
-    return _watcher(device).word.data_ptr()
+# ---- calls that are made many times a millisecond (packed_attention, layer_norm, clip_grad_norm_) ----
+# Host time per call counts there, so the device is a plain index, the stream is
+# read as a raw handle, and the status word is copied at most once a millisecond.
+_NOTE_EVERY = 1e-3  # seconds
+CHECK_STATUS = os.environ.get("MEA_CHECK_STATUS", "0") == "1"
+raw_stream = torch._C._cuda_getCurrentRawStream  # current stream's handle of device index
 
 
-def note_status_eager(device: torch.device) -> None:
-    """note_status, except in a stream capture: the event behind the copy would
-    belong to the graph, and a replay's error stays in the word until the next
-    eager call copies it."""
-    if not torch.cuda.is_current_stream_capturing():
-        _watcher(device).note()
+def status_word(idx: int) -> int:
+    """Address of the status word of device `idx`.  It is allocated by the first
+    call on the device, which must not be a captured one: the word would belong
+    to that graph's memory."""
+    w = _watch.get(idx)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device must come before a stream capture "
+                               "(it allocates the device's status word)")
+        w = _watcher(torch.device("cuda", idx))
+    return w.address
 
 
-def poll_status_eager(device: torch.device) -> None:
-    """poll_status, except in a stream capture (an event query would end it)."""
-    if not torch.cuda.is_current_stream_capturing():
-        poll_status(device)
+def after_launch(idx: int) -> None:
+    """Device-failure reporting behind a launch on device `idx`: raises what the
+    last status copy says if it has landed, and queues the next copy, at most
+    once a millisecond; check_device_status() covers the launches in between.
+    In a capture nothing is queued (a replay's error stays in the word until the
+    next eager call)."""
+    w = _watch[idx]
+    w.pending = True
+    now = time.monotonic()
+    if now < w.next_note and not CHECK_STATUS:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        return
+    w.next_note = now + _NOTE_EVERY
+    if CHECK_STATUS:
+        read_status(torch.device("cuda", idx))
+        return
+    v = w.take(block=False)
+    w.note()
+    if v != 0:
+        raise _timeout_error(v, "in an earlier call")
 
 
-class _SameDevice:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+def require_index(idx: int) -> None:
+    """require_device by device index."""
+    if idx not in _checked_devices:
+        require_device(torch.device("cuda", idx))
 
 
-_SAME_DEVICE = _SameDevice()
-
-
-def on_device(device: torch.device):
-    """Context with `device` current; nothing is switched when it already is."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _SAME_DEVICE
-    return torch.cuda.device(device)
+def launch(idx: int, fn, *args) -> None:
+    """check(fn(*args, stream)) with device `idx` current and its current stream."""
+    if torch._C._cuda_getDevice() == idx:
+        check(fn(*args, raw_stream(idx)))
+    else:
+        with torch.cuda.device(idx):
+            check(fn(*args, raw_stream(idx)))
 
 
 def check_device_status(device: torch.device | None = None) -> None:
@@ -278,7 +301,12 @@ def check_device_status(device: torch.device | None = None) -> None:
     up a bounded wait.  Call it where the caller synchronises anyway (end of an
     epoch, before a checkpoint) to see a timeout of the very last call."""
     dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
-    v = _watcher(dev).take(block=True)
+    w = _watcher(dev)
+    if w.pending:  # launches since the last copy, on whatever stream
+        with torch.cuda.device(dev):
+            torch.cuda.synchronize()
+            w.note()
+    v = w.take(block=True)
     if v != 0:
         raise _timeout_error(v, "in an earlier call")
 

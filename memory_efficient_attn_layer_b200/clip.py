@@ -24,34 +24,35 @@ def _kind(norm_type) -> int:
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype not in _lib.DTYPE_CODES or t.layout != torch.strided:
+    if t.dtype not in _lib.DTYPE_CODES or t.layout is not torch.strided:
         raise TypeError(f"gradients must be dense bf16, fp16 or fp32 tensors, got {t.dtype} ({t.layout})")
     return t.contiguous()  # t itself where it already is
 
 
 def _arrays(tensors):
-    """(count, pointers, element counts, type codes) for the C call; every tensor contiguous, on one device."""
-    device, seen = tensors[0].device, set()
-    _lib.require_device(device)
-    ptrs, ns, codes = [], [], []
+    """(device index, (count, pointers, element counts, type codes) for the C call) of contiguous tensors."""
+    idx = tensors[0].get_device()
+    if idx < 0:
+        _lib.require_device(tensors[0].device)
+    _lib.require_index(idx)
+    ptrs = [t.data_ptr() for t in tensors]
+    ns = [t.numel() for t in tensors]
     for t in tensors:
-        if t.device != device:
+        if t.get_device() != idx:
             raise ValueError("all gradients must be on the same device")
-        p, n = t.data_ptr(), t.numel()
-        if n:
-            if p in seen:
-                raise ValueError("a gradient appears twice")
-            seen.add(p)
-        ptrs.append(p)
-        ns.append(n)
-        codes.append(_lib.DTYPE_CODES[t.dtype])
     k = len(tensors)
-    return k, (ctypes.c_void_p * k)(*ptrs), (ctypes.c_longlong * k)(*ns), (ctypes.c_int * k)(*codes)
+    if len(set(ptrs)) < k:  # tensors without elements have no address of their own
+        held = [p for p, n in zip(ptrs, ns) if n]
+        if len(set(held)) < len(held):
+            raise ValueError("a gradient appears twice")
+    codes = _lib.DTYPE_CODES
+    return idx, (k, (ctypes.c_void_p * k)(*ptrs), (ctypes.c_longlong * k)(*ns),
+                 (ctypes.c_int * k)(*[codes[t.dtype] for t in tensors]))
 
 
-def _workspace(k, device):
-    nbytes = _lib.lib().mea_grad_norm_workspace_size(k)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+def _workspace(like, k):
+    """Workspace of a k-tensor call, on `like`'s device."""
+    return torch.empty(_lib.lib().mea_grad_norm_workspace_size(k), dtype=torch.uint8, device=like.device)
 
 
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -61,17 +62,13 @@ def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.
     tensors = [_dense(t) for t in tensors]
     if not tensors:
         return torch.tensor(0.0)
-    k, ptrs, ns, codes = _arrays(tensors)
-    device = tensors[0].device
-    out = torch.empty((), dtype=torch.float32, device=device)
-    with _lib.on_device(device):
-        ws, nbytes = _workspace(k, device)
-        _lib.check(_lib.lib().mea_grad_norm(k, ptrs, ns, codes, kind, out.data_ptr(), None, ws.data_ptr(), nbytes,
-                                            _lib.stream_ptr(device)))
+    idx, arrays = _arrays(tensors)
+    out = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    ws = _workspace(out, arrays[0])
+    _lib.launch(idx, _lib.lib().mea_grad_norm, *arrays, kind, out.data_ptr(), None, ws.data_ptr(), ws.numel())
     return out
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Multiplies the gradients of ``parameters`` (a tensor or an iterable; those without ``.grad`` are passed over) in
     place by min(1, max_norm / (norm + 1e-6)), where norm is the global norm of them all, and returns that norm: a 0-dim
@@ -85,22 +82,20 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for g in (p.grad for p in parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
     work = [_dense(g) for g in grads]
-    k, ptrs, ns, codes = _arrays(work)
-    device = work[0].device
+    idx, arrays = _arrays(work)
     if error_if_nonfinite:
         norm = grad_norm(work, norm_type)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"the total norm of order {norm_type} of the gradients is non-finite, so they cannot be clipped")
-    out = torch.empty((), dtype=torch.float32, device=device)
-    with _lib.on_device(device):
-        ws, nbytes = _workspace(k, device)
-        _lib.check(_lib.lib().mea_clip_grad_norm(k, ptrs, ns, codes, kind, max_norm, out.data_ptr(), ws.data_ptr(), nbytes,
-                                                 _lib.stream_ptr(device)))
-        for g, w in zip(grads, work):
-            if g is not w:
+    out = torch.empty((), dtype=torch.float32, device=work[0].device)
+    ws = _workspace(out, arrays[0])
+    _lib.launch(idx, _lib.lib().mea_clip_grad_norm, *arrays, kind, max_norm, out.data_ptr(), ws.data_ptr(), ws.numel())
+    for g, w in zip(grads, work):
+        if g is not w:
+            with torch.no_grad():
                 g.copy_(w)
     return out

@@ -56,89 +56,106 @@ __device__ __forceinline__ int seq_of(const int* pre, int n_seqs, int id) {
   return lo;
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __restrict__ cu, int n_seqs, int total,
-                                                                   int tt, int cap_q, int cap_k, PackedHeader* head,
-                                                                   int4* q_items, int4* k_items, int* scratch,
-                                                                   int* status) {
-  __shared__ int pre_s[2 * PLAN_SMEM_SEQS];
+// Block 0 lists the query tiles, block 1 the key tiles.  `at_once`: up to this
+// many tiles of the kind start together whatever their order, so they are not sorted.
+struct PlanParams {
+  int n_seqs, total, tt;
+  int cap[2], at_once[2];
+  int4* items[2];
+  PackedHeader* head;
+  int* scratch;
+  int* status;
+};
+
+__global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __restrict__ cu, const PlanParams p) {
+  __shared__ int pre_s[PLAN_SMEM_SEQS];
   __shared__ int hist[PLAN_CLASSES];
   __shared__ int warp_sums[32];
   __shared__ int longest_s;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, kind = blockIdx.x, n_seqs = p.n_seqs, tt = p.tt;
   pdl_launch();
   if (tid == 0) longest_s = 0;
-
+  const int rows = kind ? 128 : tt;  // tokens of a tile
+  int* pre = n_seqs <= PLAN_SMEM_SEQS ? pre_s : p.scratch + kind * n_seqs;
+  int n = 0, longest = 0;
+  bool good = true;
+  for (int s0 = 0; s0 < n_seqs; s0 += PLAN_THREADS) {
+    const int s = s0 + tid;
+    int tiles = 0;
+    if (s < n_seqs) {
+      const int a = cu[s], b = cu[s + 1];
+      good &= a >= 0 && a <= b && b <= p.total;
+      if (good) {
+        longest = max(longest, b - a);
+        tiles = (b - a + rows - 1) / rows;
+      }
+    }
+    int sum;
+    const int at = block_scan(tiles, warp_sums, &sum);
+    if (s < n_seqs) pre[s] = n + at;
+    n += sum;
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if ((tid & 31) == 0) atomicMax(&longest_s, longest);
   // cu_seqlens must rise from >= 0 to <= total; otherwise no tile is made (every
   // output row is then zero) and the status word says so.
-  bool good = true;
-  for (int i = tid; i < n_seqs; i += PLAN_THREADS) good &= cu[i] >= 0 && cu[i] <= cu[i + 1] && cu[i + 1] <= total;
   if (!__syncthreads_and(good)) {
     if (tid == 0) {
-      record_error(status, KID_PACKED_PLAN, 1);
-      *head = PackedHeader{0, 0, 0, 0, {0, 0, 0, 0}};
+      if (kind == 0) {
+        record_error(p.status, KID_PACKED_PLAN, 1);
+        p.head->n_q = 0;
+        p.head->first = p.head->end = 0;
+      } else {
+        p.head->n_k = 0;
+      }
     }
     return;
   }
-
-  int* pre_q = n_seqs <= PLAN_SMEM_SEQS ? pre_s : scratch;
-  int* pre_k = pre_q + (n_seqs <= PLAN_SMEM_SEQS ? PLAN_SMEM_SEQS : n_seqs);
-  int n_q = 0, n_k = 0, longest = 0;
-  for (int s0 = 0; s0 < n_seqs; s0 += PLAN_THREADS) {
-    const int s = s0 + tid;
-    const int len = s < n_seqs ? cu[s + 1] - cu[s] : 0;
-    longest = max(longest, len);
-    int sum_q, sum_k;
-    const int at_q = block_scan(int((long long)(len + tt - 1) / tt), warp_sums, &sum_q);
-    const int at_k = block_scan((len + 127) >> 7, warp_sums, &sum_k);
-    if (s < n_seqs) {
-      pre_q[s] = n_q + at_q;
-      pre_k[s] = n_k + at_k;
-    }
-    n_q += sum_q;
-    n_k += sum_k;
-  }
-  atomicMax(&longest_s, longest);
-  __syncthreads();
   longest = longest_s;
-  if (tid == 0) *head = PackedHeader{min(n_q, cap_q), min(n_k, cap_k), cu[0], cu[n_seqs], {0, 0, 0, 0}};
+  const int cap = p.cap[kind];
+  if (tid == 0) {
+    if (kind == 0) {
+      p.head->n_q = min(n, cap);
+      p.head->first = cu[0];
+      p.head->end = cu[n_seqs];
+    } else {
+      p.head->n_k = min(n, cap);
+    }
+  }
 
-#pragma unroll 1
-  for (int kind = 0; kind < 2; ++kind) {  // query tiles, then key tiles
-    const int* pre = kind ? pre_k : pre_q;
-    const int n = kind ? n_k : n_q, cap = kind ? cap_k : cap_q;
-    int4* items = kind ? k_items : q_items;
-    const int most = kind ? (longest + tt - 1) / tt : (longest + 127) >> 7;  // steps of the longest tile
-    int shift = 0;
-    while ((most >> shift) >= PLAN_CLASSES) ++shift;
-    auto item = [&](int id, int& cls) {
-      const int s = seq_of(pre, n_seqs, id);
-      const int begin = cu[s], len = cu[s + 1] - begin, tile = id - pre[s];
-      // steps: key tiles up to the query tile's last token, or query tiles from the key tile's first
-      const int steps = kind ? (len + tt - 1) / tt - tile * 128 / tt
-                             : (int(min((long long)(tile + 1) * tt, (long long)len)) + 127) >> 7;
-      cls = (most >> shift) - (steps >> shift);
-      return make_int4(begin, len, tile, 0);
-    };
-    hist[tid] = 0;
-    __syncthreads();
-    for (int id = tid; id < n; id += PLAN_THREADS) {
-      int cls;
-      item(id, cls);
-      atomicAdd(&hist[cls], 1);
-    }
-    __syncthreads();
-    int all;
-    const int at = block_scan(hist[tid], warp_sums, &all);
-    __syncthreads();
-    hist[tid] = at;
-    __syncthreads();
-    for (int id = tid; id < n; id += PLAN_THREADS) {
-      int cls;
-      const int4 it = item(id, cls);
-      const int slot = atomicAdd(&hist[cls], 1);  // order within a class is free: tiles are independent
-      if (slot < cap) items[slot] = it;
-    }
-    __syncthreads();
+  int4* items = p.items[kind];
+  const int most = kind ? (longest + tt - 1) / tt : (longest + 127) >> 7;  // steps of the longest tile
+  int shift = 0;
+  while ((most >> shift) >= PLAN_CLASSES) ++shift;
+  auto item = [&](int id, int& cls) {
+    const int s = seq_of(pre, n_seqs, id);
+    const int begin = cu[s], len = cu[s + 1] - begin, tile = id - pre[s];
+    // steps: key tiles up to the query tile's last token, or query tiles from the key tile's first
+    const int steps = kind ? (len + tt - 1) / tt - tile * 128 / tt
+                           : (int(min((long long)(tile + 1) * tt, (long long)len)) + 127) >> 7;
+    cls = (most >> shift) - (steps >> shift);
+    return make_int4(begin, len, tile, 0);
+  };
+  int cls;
+  if (n <= p.at_once[kind]) {
+    for (int id = tid; id < min(n, cap); id += PLAN_THREADS) items[id] = item(id, cls);
+    return;
+  }
+  hist[tid] = 0;
+  __syncthreads();
+  for (int id = tid; id < n; id += PLAN_THREADS) {
+    item(id, cls);
+    atomicAdd(&hist[cls], 1);
+  }
+  __syncthreads();
+  int all;
+  const int at = block_scan(hist[tid], warp_sums, &all);
+  hist[tid] = at;
+  __syncthreads();
+  for (int id = tid; id < n; id += PLAN_THREADS) {
+    const int4 it = item(id, cls);
+    const int slot = atomicAdd(&hist[cls], 1);  // order within a class is free: tiles are independent
+    if (slot < cap) items[slot] = it;
   }
 }
 static_assert(PLAN_CLASSES == PLAN_THREADS, "one class per thread in the scan");
@@ -151,6 +168,8 @@ int packed_dims(const mea_packed_dims* d, PackedDims* out) {
   if (d->total < 0 || d->n_seqs < 0)
     return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: total=%d and n_seqs=%d must be >= 0", d->total,
                      d->n_seqs);
+  if (d->total > (1 << 30))
+    return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention: total=%d is more than 2^30 rows", d->total);
   if (d->Hq <= 0 || d->Hkv <= 0 || d->Hq % d->Hkv)
     return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention: Hq=%d must be a positive multiple of Hkv=%d", d->Hq,
                      d->Hkv);
@@ -207,9 +226,20 @@ int run_packed_plan(const PackedDims& d, const int* cu, void* plan, int* status,
   const PackedPlan v = packed_plan_view(d, plan);
   char* scratch = static_cast<char*>(plan) + up256(sizeof(PackedHeader)) + up256(sizeof(int4) * size_t(d.cap_q)) +
                   up256(sizeof(int4) * size_t(d.cap_k));
-  packed_plan_kernel<<<1, PLAN_THREADS, 0, st>>>(cu, d.n_seqs, d.total, d.tt, d.cap_q, d.cap_k,
-                                                 const_cast<PackedHeader*>(v.head), const_cast<int4*>(v.q_items),
-                                                 const_cast<int4*>(v.k_items), reinterpret_cast<int*>(scratch), status);
+  PlanParams p;
+  p.n_seqs = d.n_seqs;
+  p.total = d.total;
+  p.tt = d.tt;
+  p.cap[0] = d.cap_q;
+  p.cap[1] = d.cap_k;
+  p.at_once[0] = num_sms() / d.hg;  // times hg head groups: one CTA an SM in the dQ kernel
+  p.at_once[1] = num_sms() / d.Hkv;
+  p.items[0] = const_cast<int4*>(v.q_items);
+  p.items[1] = const_cast<int4*>(v.k_items);
+  p.head = const_cast<PackedHeader*>(v.head);
+  p.scratch = reinterpret_cast<int*>(scratch);
+  p.status = status;
+  packed_plan_kernel<<<2, PLAN_THREADS, 0, st>>>(cu, p);
   return check_launch("packed_plan_kernel");
 }
 

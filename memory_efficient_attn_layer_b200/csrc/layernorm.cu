@@ -12,12 +12,14 @@
 // so dw and db grow in registers; each block writes one fp32 partial row and a
 // second kernel adds those in a fixed order.  All sums are fp32.
 //
-// Rows too long for that (above 16384 elements) take kernels that walk the row
-// several times, and a column-wise pass for dw and db.
+// Rows too long for that (above 16384 elements; 8192 in the backward where they
+// are not whole 16-byte vectors) take kernels that walk the row several times,
+// and a column-wise pass for dw and db.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "launch.h"
 #include "ptx.cuh"
@@ -165,10 +167,37 @@ __global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_fwd_kernel(long l
   }
 }
 
-// R rows per group and round; block i takes every gridDim.x-th round.  Partial
-// sums of the block's rows: part[(2 i) C ..] for dw, part[(2 i + 1) C ..] for db.
+// What one thread holds of a row before it is converted: 16 bytes, or one element.
+template <class T, int VEC>
+struct Raw {
+  uint4 r;
+  __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void clear() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ float operator[](int e) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[e]);
+    } else {
+      const uint32_t h = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(h << 16);
+      return __half2float(__ushort_as_half(uint16_t(h)));
+    }
+  }
+};
+template <class T>
+struct Raw<T, 1> {
+  T r;
+  __device__ __forceinline__ void load(const T* p) { r = *p; }
+  __device__ __forceinline__ void clear() { r = from_f<T>(0.f); }
+  __device__ __forceinline__ float operator[](int) const { return to_f(r); }
+};
+
+// R rows per group and round; block i takes every gridDim.x-th round, and the
+// next round's rows are on their way while this one's are summed (they wait as
+// they lie in memory, so the second set costs few registers).  Partial sums of
+// the block's rows: part[(2 i) C ..] for dw, part[(2 i + 1) C ..] for db.
 template <class T, class W, int VEC, int TPR, int V, int R>
-__global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_bwd_kernel(long long rows, int C,
+__global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) layernorm_bwd_kernel(long long rows, int C,
                                                                          const T* __restrict__ dy,
                                                                          const T* __restrict__ x,
                                                                          const W* __restrict__ w,
@@ -193,8 +222,11 @@ __global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_bwd_kernel(long l
     }
     if (w && c < C) load_vec<VEC>(w + c, ww[v]);
   }
-  for (long long row0 = (long long)blockIdx.x * GROUPS * R; row0 < rows; row0 += (long long)gridDim.x * GROUPS * R) {
-    float xf[R][V][VEC], df[R][V][VEC], rstd[R], sums[2 * R];
+  struct Rows {
+    Raw<T, VEC> x[R][V], d[R][V];
+    float mean[R], rstd[R];
+  };
+  auto fetch = [&](Rows& a, long long row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + g * R + r;
@@ -202,31 +234,40 @@ __global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_bwd_kernel(long l
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int c = (v * TPR + lane) * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) xf[r][v][e] = df[r][v][e] = 0.f;
         if (live && c < C) {
-          load_vec<VEC>(x + row * C + c, xf[r][v]);
-          load_vec<VEC>(dy + row * C + c, df[r][v]);
+          a.x[r][v].load(x + row * C + c);
+          a.d[r][v].load(dy + row * C + c);
+        } else {
+          a.x[r][v].clear();
+          a.d[r][v].clear();
         }
       }
-      rstd[r] = live ? rstd_in[row] : 0.f;
+      a.mean[r] = live ? mean_in[row] : 0.f;
+      a.rstd[r] = live ? rstd_in[row] : 0.f;  // xhat = 0 in rows that are not there
     }
+  };
+  const long long step = (long long)gridDim.x * GROUPS * R;
+  long long row0 = (long long)blockIdx.x * GROUPS * R;
+  Rows a;
+  if (row0 < rows) fetch(a, row0);
+  for (; row0 < rows; row0 += step) {
+    Rows next;
+    if (row0 + step < rows) fetch(next, row0 + step);
+    float sums[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const long long row = row0 + g * R + r;
-      const float mean = row < rows ? mean_in[row] : 0.f;
       sums[2 * r] = sums[2 * r + 1] = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if ((v * TPR + lane) * VEC >= C) continue;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          xf[r][v][e] = (xf[r][v][e] - mean) * rstd[r];
-          const float gg = df[r][v][e] * ww[v][e];
+          const float xh = (a.x[r][v][e] - a.mean[r]) * a.rstd[r], d = a.d[r][v][e];
+          const float gg = d * ww[v][e];
           sums[2 * r] += gg;
-          sums[2 * r + 1] += gg * xf[r][v][e];
-          dw[v][e] += df[r][v][e] * xf[r][v][e];
-          db[v][e] += df[r][v][e];
+          sums[2 * r + 1] += gg * xh;
+          dw[v][e] += d * xh;
+          db[v][e] += d;
         }
       }
     }
@@ -242,10 +283,12 @@ __global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_bwd_kernel(long l
         if (c >= C) continue;
         float o[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = rstd[r] * (df[r][v][e] * ww[v][e] - m1 - xf[r][v][e] * m2);
+        for (int e = 0; e < VEC; ++e)
+          o[e] = a.rstd[r] * (a.d[r][v][e] * ww[v][e] - m1 - (a.x[r][v][e] - a.mean[r]) * a.rstd[r] * m2);
         store_vec<VEC>(dx + row * C + c, o);
       }
     }
+    a = next;
   }
   if (!part) return;
   float* out = part + (long long)blockIdx.x * 2 * C;
@@ -383,17 +426,38 @@ __global__ void __launch_bounds__(256) layernorm_part_long_kernel(long long rows
 struct LnShape {
   int vec, tpr, v;  // v = 0: the long-row kernels
 };
-static LnShape ln_shape(int C, int elem, bool aligned) {
+// Forward: one warp per row while it holds it in 8 vectors a lane (32 single
+// elements), because then no barrier stands between the row's load and its store;
+// longer rows take more warps, and so do rows too few to give every SM a block.
+static LnShape ln_fwd_shape(long long rows, int C, int elem, bool aligned) {
+  LnShape s;
+  s.vec = aligned && C % (16 / elem) == 0 ? 16 / elem : 1;
+  const int units = (C + s.vec - 1) / s.vec, least = s.vec == 1 ? 8 : 1, most = s.vec == 1 ? 32 : 8;
+  s.tpr = 32;
+  while (s.tpr < 512 && s.tpr * most < units) s.tpr *= 2;
+  s.v = least;
+  while (s.tpr * s.v < units) s.v *= s.vec == 1 ? 4 : 2;
+  if (s.v > most) {
+    s.v = 0;
+    return s;
+  }
+  while (s.vec > 1 && s.v > least && s.tpr < 256 && rows * s.tpr < (long long)num_sms() * 256) {
+    s.tpr *= 2;
+    s.v /= 2;
+  }
+  return s;
+}
+// Backward: a thread also keeps two sums per column, so TPR grows before V.
+static LnShape ln_bwd_shape(int C, int elem, bool aligned) {
   LnShape s;
   s.vec = aligned && C % (16 / elem) == 0 ? 16 / elem : 1;
   const int units = (C + s.vec - 1) / s.vec;
   s.tpr = 32;
   const int most = s.vec == 1 ? 8 : 1;  // vectors (or single elements) a thread takes before the next doubling of TPR
   while (s.tpr < 512 && s.tpr * most < units) s.tpr *= 2;
-  s.v = 1;
+  s.v = most;
   while (s.tpr * s.v < units) s.v *= 2;
-  if (s.vec == 1 && s.v < 8) s.v = 8;
-  if (s.vec * s.v > 32) s.v = 0;
+  if (s.vec * s.v > (s.vec == 1 ? 16 : 32)) s.v = 0;
   return s;
 }
 constexpr int LN_LONG_PARTS = 64;
@@ -403,10 +467,10 @@ static int ln_bwd_blocks(long long rows, const LnShape& s, int rows_per_round) {
   const long long rounds = (rows + (long long)groups * rows_per_round - 1) / ((long long)groups * rows_per_round);
   return int(std::min<long long>(rounds, (long long)num_sms() * (threads > 256 ? 1 : 2)));
 }
-// Rows in flight per group: as many as keep the row registers (x and dy) near 64.
+// Rows per group and round; two rounds are in flight, 16 bytes of x and of dy per vector.
 template <int VEC, int V>
 constexpr int ln_rows() {
-  return VEC * V >= 32 ? 1 : VEC * V >= 16 ? 2 : 4;
+  return VEC * V > 8 ? 1 : VEC == 1 ? 2 : 4;
 }
 
 template <class T, class W, int VEC, int TPR, int V>
@@ -429,29 +493,50 @@ static void ln_bwd(long long rows, int C, const void* dy, const void* x, const v
       static_cast<T*>(dx), part);
 }
 
-// Calls f.template run<VEC, TPR, V>() for the shape: with 16-byte vectors TPR
-// grows first (V = 1 below TPR = 512); with single elements V = 8 below that.
+// f(VEC, TPR, V) as compile-time constants for a shape of ln_fwd_shape.
 template <int FULL, class F>
-static void ln_dispatch(const LnShape& s, F&& f) {
+static void ln_fwd_dispatch(const LnShape& s, F&& f) {
+  using std::integral_constant;
   auto tpr = [&](auto vec, auto v) {
     switch (s.tpr) {
-      case 32: f(vec, std::integral_constant<int, 32>(), v); break;
-      case 64: f(vec, std::integral_constant<int, 64>(), v); break;
-      case 128: f(vec, std::integral_constant<int, 128>(), v); break;
-      case 256: f(vec, std::integral_constant<int, 256>(), v); break;
-      default: f(vec, std::integral_constant<int, 512>(), v); break;
+      case 32: return f(vec, integral_constant<int, 32>(), v);
+      case 64: return f(vec, integral_constant<int, 64>(), v);
+      case 128: return f(vec, integral_constant<int, 128>(), v);
+      case 256: return f(vec, integral_constant<int, 256>(), v);
+      default: return f(vec, integral_constant<int, 512>(), v);
     }
   };
+  if (s.vec == 1) return s.v == 8 ? tpr(integral_constant<int, 1>(), integral_constant<int, 8>())
+                                  : tpr(integral_constant<int, 1>(), integral_constant<int, 32>());
+  integral_constant<int, FULL> vec;
+  switch (s.v) {
+    case 1: return tpr(vec, integral_constant<int, 1>());
+    case 2: return tpr(vec, integral_constant<int, 2>());
+    case 4: return tpr(vec, integral_constant<int, 4>());
+    default: return tpr(vec, integral_constant<int, 8>());
+  }
+}
+// The same for ln_bwd_shape: V is above its least value at TPR = 512 only.
+template <int FULL, class F>
+static void ln_bwd_dispatch(const LnShape& s, F&& f) {
   using std::integral_constant;
+  auto tpr = [&](auto vec, auto v) {
+    switch (s.tpr) {
+      case 32: return f(vec, integral_constant<int, 32>(), v);
+      case 64: return f(vec, integral_constant<int, 64>(), v);
+      case 128: return f(vec, integral_constant<int, 128>(), v);
+      case 256: return f(vec, integral_constant<int, 256>(), v);
+      default: return f(vec, integral_constant<int, 512>(), v);
+    }
+  };
+  integral_constant<int, 512> all;
   if (s.vec == 1) {
     integral_constant<int, 1> one;
     if (s.v == 8) return tpr(one, integral_constant<int, 8>());
-    integral_constant<int, 512> all;
-    return s.v == 16 ? f(one, all, integral_constant<int, 16>()) : f(one, all, integral_constant<int, 32>());
+    return f(one, all, integral_constant<int, 16>());
   }
   integral_constant<int, FULL> vec;
   if (s.v == 1) return tpr(vec, integral_constant<int, 1>());
-  integral_constant<int, 512> all;
   if (s.v == 2) return f(vec, all, integral_constant<int, 2>());
   if (s.v == 4) return f(vec, all, integral_constant<int, 4>());
   if constexpr (FULL == 4) f(vec, all, integral_constant<int, 8>());
@@ -466,14 +551,14 @@ static int layernorm_fwd(long long rows, int C, float eps, const void* x, const 
                                                            static_cast<const W*>(w), static_cast<const W*>(b),
                                                            static_cast<T*>(y), mean, rstd);
   } else {
-    ln_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
+    ln_fwd_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
       ln_fwd<T, W, vec(), tpr(), v()>(rows, C, eps, x, w, b, y, mean, rstd, st);
     });
   }
   return check_launch("layernorm_fwd_kernel");
 }
 
-static int ln_rows_of(const LnShape& s) { return s.vec * s.v >= 32 ? 1 : s.vec * s.v >= 16 ? 2 : 4; }
+static int ln_rows_of(const LnShape& s) { return s.vec * s.v > 8 ? 1 : s.vec == 1 ? 2 : 4; }
 
 template <class T, class W>
 static int layernorm_bwd(long long rows, int C, const void* dy, const void* x, const void* w, const float* mean,
@@ -492,7 +577,7 @@ static int layernorm_bwd(long long rows, int C, const void* dy, const void* x, c
       }
     } else {
       parts = ln_bwd_blocks(rows, s, ln_rows_of(s));
-      ln_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
+      ln_bwd_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
         ln_bwd<T, W, vec(), tpr(), v()>(rows, C, dy, x, w, mean, rstd, dx, part, parts, st);
       });
     }
@@ -557,7 +642,7 @@ extern "C" int mea_layernorm_forward(long long rows, int C, float eps, int dtype
       (rc = ln_align({w, b}, wdtype == MEA_FP32 ? 4 : 2)) != MEA_OK)
     return rc;
   auto st = static_cast<cudaStream_t>(stream);
-  const LnShape s = ln_shape(C, elem, ln_vector({x, y, w, b}));
+  const LnShape s = ln_fwd_shape(rows, C, elem, ln_vector({x, y, w, b}));
   if (dtype == MEA_FP32) return layernorm_fwd<float, float>(rows, C, eps, x, w, b, y, mean, rstd, s, st);
   if (dtype == MEA_BF16)
     return wdtype == MEA_FP32 ? layernorm_fwd<__nv_bfloat16, float>(rows, C, eps, x, w, b, y, mean, rstd, s, st)
@@ -587,7 +672,7 @@ extern "C" int mea_layernorm_backward(long long rows, int C, int dtype, int wdty
                      mea_layernorm_workspace_size(rows, C));
   auto st = static_cast<cudaStream_t>(stream);
   float* part = sums ? static_cast<float*>(workspace) : nullptr;
-  const LnShape s = ln_shape(C, elem, ln_vector({dy, x, dx, w}));
+  const LnShape s = ln_bwd_shape(C, elem, ln_vector({dy, x, dx, w}));
   if (dtype == MEA_FP32) return layernorm_bwd<float, float>(rows, C, dy, x, w, mean, rstd, dx, dw, db, part, s, st);
   if (dtype == MEA_BF16)
     return wdtype == MEA_FP32

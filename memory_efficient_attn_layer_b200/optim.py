@@ -243,11 +243,10 @@ class ShardedAdamW(torch.optim.Optimizer):
         if self.max_grad_norm is None:
             _lib.check(lib.mea_adamw_step(*args, _lib.stream_ptr(dev)))
         else:
-            with _lib.on_device(dev):
-                sumsq = self._sum_of_squares()
-                self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
-                _lib.check(lib.mea_adamw_step_clipped(*args, sumsq.data_ptr(), self.max_grad_norm,
-                                                      self.grad_norm.data_ptr(), _lib.stream_ptr(dev)))
+            sumsq = self._sum_of_squares()
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
+            _lib.launch(dev.index, lib.mea_adamw_step_clipped, *args, sumsq.data_ptr(), self.max_grad_norm,
+                        self.grad_norm.data_ptr())
         L.all_gather(self.param_shard)
         return loss
 
@@ -257,9 +256,9 @@ class ShardedAdamW(torch.optim.Optimizer):
         nbytes = lib.mea_grad_norm_workspace_size(1)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         sumsq = torch.empty((), dtype=torch.float64, device=dev)
-        _lib.check(lib.mea_grad_norm(
-            1, (ctypes.c_void_p * 1)(self.grad_shard.data_ptr()), (ctypes.c_longlong * 1)(L.shard),
-            (ctypes.c_int * 1)(_lib.MEA_FP32), 0, None, sumsq.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_ptr(dev)))
+        _lib.launch(dev.index, lib.mea_grad_norm, 1, (ctypes.c_void_p * 1)(self.grad_shard.data_ptr()),
+                    (ctypes.c_longlong * 1)(L.shard), (ctypes.c_int * 1)(_lib.MEA_FP32), 0, None, sumsq.data_ptr(),
+                    ws.data_ptr(), nbytes)
         if L.world > 1:
             dist.all_reduce(sumsq, group=L.group)
         return sumsq

@@ -15,6 +15,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
+_CODES = {torch.bfloat16: _lib.MEA_BF16, torch.float16: _lib.MEA_FP16}
+
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` ([total, heads, N]) if the kernels can read it in place (heads' values contiguous, row and head strides
@@ -27,7 +29,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _check(q, k, v, cu_seqlens, scale):
+def _refuse(q, k, v, cu_seqlens, scale):
+    """Raises what is wrong with the arguments."""
     _lib.require_device(q.device)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be [total, heads, N], got shapes "
@@ -40,16 +43,71 @@ def _check(q, k, v, cu_seqlens, scale):
         raise ValueError(f"the query heads ({hq}) must be a positive multiple of the key/value heads ({hkv})")
     if n == 0 or n % 8 or n > 128:
         raise ValueError(f"the head dim must be a multiple of 8 up to 128, got {n}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    if q.dtype not in _CODES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("packed_attention computes in bf16 or fp16, one type for all of q, k and v; got "
                         f"{q.dtype}, {k.dtype}, {v.dtype}")
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise TypeError("cu_seqlens must be a one-dimensional int32 tensor of n_seqs + 1 row numbers, got "
                         f"{cu_seqlens.dtype} of shape {tuple(cu_seqlens.shape)}")
-    if k.device != q.device or v.device != q.device or cu_seqlens.device != q.device:
-        raise ValueError("all tensors must be on the same device")
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
+    raise ValueError("all tensors must be on the same device")
+
+
+def _forward(q, k, v, cu_seqlens, scale):
+    """(o, what the backward needs besides q, k, v and o: their readable forms, the row log-sum-exp and the plan)."""
+    dt, idx = q.dtype, q.get_device()
+    if not (idx >= 0 and k.get_device() == idx and v.get_device() == idx and cu_seqlens.get_device() == idx
+            and dt in _CODES and k.dtype is dt and v.dtype is dt and cu_seqlens.dtype is torch.int32
+            and q.dim() == 3 and k.dim() == 3 and v.dim() == 3 and cu_seqlens.dim() == 1 and 0.0 < scale < 3e38):
+        _refuse(q, k, v, cu_seqlens, scale)
+    total, hq, n = q.shape
+    total_k, hkv, n_k = k.shape
+    n_seqs = cu_seqlens.numel() - 1
+    if (k.shape != v.shape or total_k != total or n_k != n or hkv == 0 or hq == 0 or hq % hkv or n == 0 or n % 8 or n > 128
+            or n_seqs < 0):
+        _refuse(q, k, v, cu_seqlens, scale)
+    _lib.require_index(idx)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if not cu_seqlens.is_contiguous():
+        cu_seqlens = cu_seqlens.contiguous()
+    dims = _lib.MeaPackedDims(total, n_seqs, hq, hkv, n, _CODES[dt], scale, *q.stride()[:2], *k.stride()[:2],
+                              *v.stride()[:2])
+    o = q.new_empty((total, hq, n))
+    if total == 0:
+        return o, (q, k, v, None), dims
+    L = _lib.lib()
+    at = ctypes.byref(dims)
+    nbytes = L.mea_packed_plan_size(at)
+    # one buffer: the plan, then lse2 [total, Hq] fp32, then the backward's delta of the same size
+    rows = 4 * total * hq
+    side = torch.empty(nbytes + 2 * rows, dtype=torch.uint8, device=q.device)
+    p = side.data_ptr()
+    _lib.launch(idx, L.mea_packed_attention_forward, at, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(),
+                o.data_ptr(), p + nbytes, p, nbytes, _lib.status_word(idx))
+    _lib.after_launch(idx)
+    return o, (q, k, v, side), dims
+
+
+def _backward(ctx, grad_output):
+    q, k, v, o, side = ctx.saved_tensors
+    dq = q.new_empty(q.shape)
+    dk = k.new_empty(k.shape)
+    dv = k.new_empty(k.shape)
+    if side is None:
+        return dq, dk, dv, None, None
+    do = _rows(grad_output)
+    idx, p = q.get_device(), side.data_ptr()
+    rows = 4 * q.shape[0] * q.shape[1]
+    nbytes = side.numel() - 2 * rows
+    _lib.launch(idx, _lib.lib().mea_packed_attention_backward, ctypes.byref(ctx.dims), q.data_ptr(), k.data_ptr(),
+                v.data_ptr(), o.data_ptr(), do.data_ptr(), *do.stride()[:2], p + nbytes, p, nbytes, p + nbytes + rows,
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.status_word(idx))
+    _lib.after_launch(idx)
+    return dq, dk, dv, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class PackedAttentionFunction(torch.autograd.Function):
@@ -58,50 +116,14 @@ class PackedAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, scale):
-        _check(q, k, v, cu_seqlens, scale)
-        q, k, v, cu_seqlens = _rows(q), _rows(k), _rows(v), cu_seqlens.contiguous()
-        total, hq, n = q.shape
-        dims = _lib.MeaPackedDims(total, cu_seqlens.numel() - 1, hq, k.shape[1], n, _lib.DTYPE_CODES[q.dtype], scale,
-                                  q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        o = torch.empty(total, hq, n, dtype=q.dtype, device=q.device)
-        if total == 0:
-            lse = plan = None
-        else:
-            with _lib.on_device(q.device):
-                _lib.poll_status_eager(q.device)
-                L = _lib.lib()
-                nbytes = L.mea_packed_plan_size(ctypes.byref(dims))
-                lse = torch.empty(total, hq, dtype=torch.float32, device=q.device)
-                plan = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-                _lib.check(L.mea_packed_attention_forward(
-                    ctypes.byref(dims), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), o.data_ptr(),
-                    lse.data_ptr(), plan.data_ptr(), nbytes, _lib.status_word(q.device),
-                    _lib.stream_ptr(q.device)))
-                _lib.note_status_eager(q.device)
-        ctx.save_for_backward(q, k, v, o, lse, plan)
-        ctx.dims = dims
+        o, (q, k, v, side), ctx.dims = _forward(q, k, v, cu_seqlens, scale)
+        ctx.save_for_backward(q, k, v, o, side)
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_output):
-        q, k, v, o, lse, plan = ctx.saved_tensors
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        if q.shape[0] == 0:
-            return dq, dk, dv, None, None
-        do = _rows(grad_output)
-        with _lib.on_device(q.device):
-            _lib.poll_status_eager(q.device)
-            delta = torch.empty_like(lse)
-            _lib.check(_lib.lib().mea_packed_attention_backward(
-                ctypes.byref(ctx.dims), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(),
-                do.stride(0), do.stride(1), lse.data_ptr(), plan.data_ptr(), plan.numel(), delta.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.status_word(q.device),
-                _lib.stream_ptr(q.device)))
-            _lib.note_status_eager(q.device)
-        return dq, dk, dv, None, None
+        # The gradients have no derivative of their own; the marking costs host time, so only where one could be taken.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_output)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -118,4 +140,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     nothing is copied to the host, and a captured call follows the values that ``cu_seqlens`` has at each replay.  A
     ``cu_seqlens`` that does not rise from >= 0 to <= total gives zeros and a MeaError at a later call or at
     ``check_device_status()``.  The same call gives the same bits."""
-    return PackedAttentionFunction.apply(q, k, v, cu_seqlens, float(q.shape[-1] ** -0.5 if scale is None else scale))
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return PackedAttentionFunction.apply(q, k, v, cu_seqlens, scale)
+    return _forward(q, k, v, cu_seqlens, scale)[0]

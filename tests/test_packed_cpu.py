@@ -81,7 +81,7 @@ def _dims(total=256, n_seqs=2, hq=8, hkv=2, n=64, dtype=0, scale=0.125, **stride
     (dict(scale=0.0), 1, b"scale"),
     (dict(scale=float("nan")), 1, b"scale"),
     (dict(scale=float("inf")), 1, b"scale"),
-    (dict(total=2**31 - 1, hq=4096, hkv=4096), 2, b"too many tiles"),
+    (dict(total=2**30, hq=4096, hkv=4096), 2, b"too many tiles"), (dict(total=2**30 + 1), 2, b"2^30 rows"),
 ])
 def test_sizes_are_refused(kw, code, text):
     L = _lib.lib()
