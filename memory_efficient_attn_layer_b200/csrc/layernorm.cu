@@ -10,10 +10,14 @@
 // about the mean (a second sum, not a difference of large ones).  In the
 // backward each thread keeps its own columns for every row that its block takes,
 // so dw and db grow in registers; each block writes one fp32 partial row and a
-// second kernel adds those in a fixed order.  All sums are fp32.
+// second kernel adds those in a fixed order.  All sums are fp32.  Either way the
+// next rows' loads are in flight while the present ones are summed: 65536 x 2048
+// bf16 takes 92 us forward (5.8 TB/s) and 155 us backward with its column sums
+// (5.2 TB/s); without the second set of rows 106 and 185 us.
 //
-// Rows too long for that (above 16384 elements; 8192 in the backward where they
-// are not whole 16-byte vectors) take kernels that walk the row several times,
+// Rows too long for that (above 512 x 8 16-byte vectors forward and 512 x 32
+// elements backward; 16384 and 8192 elements where a row is no whole number of
+// vectors) take kernels that walk the row several times,
 // and a column-wise pass for dw and db.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,7 +27,6 @@
 
 #include "launch.h"
 #include "ptx.cuh"
-
 namespace mea {
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -68,30 +71,47 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
   }
 }
 
-// Sums K values over each group of TPR threads; every thread gets the sums.
-// One block barrier: `red` holds two sets, used in turn.
+// Sums K values (a power of two) over each group of TPR threads; every thread
+// gets the sums.  Within a warp the values are folded onto each other first (each
+// step halves the values a lane carries), so K sums cost about K + 5 shuffles
+// instead of 5 K.  One block barrier when a group has several warps: `red` holds
+// two sets, used in turn.
 template <int TPR, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* red, int& turn) {
+  const int lane = threadIdx.x & 31;
+  int m = 16;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int n = K / 2; n >= 1; n /= 2, m /= 2) {
+    const bool upper = lane & m;
 #pragma unroll
-    for (int m = 16; m; m >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
-  if constexpr (TPR > 32) {
+    for (int i = 0; i < n; ++i) {
+      const float give = upper ? v[i] : v[i + n];
+      v[i] = (upper ? v[i + n] : v[i]) + __shfl_xor_sync(0xffffffffu, give, m);
+    }
+  }
+  float t = v[0];
+#pragma unroll
+  for (; m; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+  // Lane l now holds the sum of value l / (32 / K).
+  if constexpr (TPR == 32) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = K == 1 ? t : __shfl_sync(0xffffffffu, t, k * (32 / K));
+  } else {
     constexpr int WARPS = TPR / 32;
     const int warp = threadIdx.x >> 5, all = blockDim.x >> 5;
     float* r = red + turn * all * K;
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int k = 0; k < K; ++k) r[warp * K + k] = v[k];
-    __syncthreads();
+    if (lane % (32 / K) == 0) r[warp * K + lane / (32 / K)] = t;
+    named_bar_sync(1 + threadIdx.x / TPR, TPR);  // the group's own threads only
     const float* first = r + (warp / WARPS) * WARPS * K;
+    t = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = 0.f;
+    for (int i = 0; i < WARPS * K; i += 32)
+      if (i + lane < WARPS * K) t += first[i + lane];  // value lane % K of several warps
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w)
+    for (int d = 16; d >= K; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += first[w * K + k];
+    for (int k = 0; k < K; ++k) v[k] = K == 1 ? t : __shfl_sync(0xffffffffu, t, k);
   }
 }
 
@@ -100,46 +120,119 @@ constexpr int ln_threads() {
   return TPR > 256 ? TPR : 256;
 }
 
+// What one thread holds of a row, as it lies in memory: V vectors of 16 bytes, or
+// V single elements.  pair(i) converts elements 2 i and 2 i + 1 (element v VEC + e
+// is column (v TPR + lane) VEC + e); columns past C hold zero.
+template <class T, int VEC, int TPR, int V>
+struct Row {
+  static constexpr int PAIRS = V * VEC / 2;
+  static_assert(VEC > 1 || V % 2 == 0, "");
+  typename std::conditional<VEC == 1, T, uint4>::type r[V];
+  __device__ __forceinline__ void load(const T* row, int lane, int C, bool live) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * TPR + lane) * VEC;
+      if constexpr (VEC == 1)
+        r[v] = live && c < C ? row[c] : from_f<T>(0.f);
+      else
+        r[v] = live && c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (VEC == 1) {
+      return make_float2(to_f(r[2 * i]), to_f(r[2 * i + 1]));
+    } else {
+      const uint4& q = r[2 * i / VEC];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      const int k = i % (VEC / 2);
+      if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(bf16_lo(w[k]), bf16_hi(w[k]));
+      return __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    }
+  }
+};
+// Stores PAIRS pairs as T at the thread's columns of `row`.
+template <class T, int VEC, int TPR, int V>
+__device__ __forceinline__ void store_row(T* row, int lane, int C, const float2 (&f)[V * VEC / 2]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (v * TPR + lane) * VEC;
+    if (c >= C) continue;
+    if constexpr (VEC == 1) {
+      row[c] = from_f<T>(v & 1 ? f[v / 2].y : f[v / 2].x);
+    } else {
+      float o[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) {
+        o[e] = f[(v * VEC + e) / 2].x;
+        o[e + 1] = f[(v * VEC + e) / 2].y;
+      }
+      store_vec<VEC>(row + c, o);
+    }
+  }
+}
+// The thread's columns of a weight vector as pairs; `none` where there is no vector or no column.
+template <class W, int VEC, int TPR, int V>
+__device__ __forceinline__ void load_cols(const W* w, int lane, int C, float none, float2 (&f)[V * VEC / 2]) {
+  float t[V * VEC];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (v * TPR + lane) * VEC;
+    float x[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[e] = none;
+    if (w && c < C) load_vec<VEC>(w + c, x);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) t[v * VEC + e] = x[e];
+  }
+#pragma unroll
+  for (int i = 0; i < V * VEC / 2; ++i) f[i] = make_float2(t[2 * i], t[2 * i + 1]);
+}
+__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
+
+template <int TPR, int ELEMS>
+constexpr int ln_fwd_blocks() {
+  constexpr int threads = ELEMS > 32 ? 640 : 768;
+  return threads / ln_threads<TPR>() ? threads / ln_threads<TPR>() : 1;
+}
 template <class T, class W, int VEC, int TPR, int V>
-__global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_fwd_kernel(long long rows, int C, float eps,
+__global__ void __launch_bounds__(ln_threads<TPR>(), ln_fwd_blocks<TPR, VEC * V>()) layernorm_fwd_kernel(long long rows, int C, float eps,
                                                                          const T* __restrict__ x,
                                                                          const W* __restrict__ w,
                                                                          const W* __restrict__ b, T* __restrict__ y,
                                                                          float* __restrict__ mean_out,
                                                                          float* __restrict__ rstd_out) {
-  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR;
+  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR, PAIRS = V * VEC / 2;
   __shared__ float red[2 * THREADS / 32];
   int turn = 0;
   const int g = threadIdx.x / TPR, lane = threadIdx.x % TPR;
   const float inv_c = 1.0f / float(C);
-  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < rows; row0 += (long long)gridDim.x * GROUPS) {
+  const long long step = (long long)gridDim.x * GROUPS;
+  long long row0 = (long long)blockIdx.x * GROUPS;
+  Row<T, VEC, TPR, V> next;
+  next.load(x + (row0 + g) * C, lane, C, row0 + g < rows);
+  for (; row0 < rows; row0 += step) {
     const long long row = row0 + g;
     const bool live = row < rows;
-    const T* xr = x + row * C;
-    float f[V][VEC];
-    float s[1] = {0.f};
+    const Row<T, VEC, TPR, V> a = next;
+    next.load(x + (row + step) * C, lane, C, row + step < rows);  // on its way while this row is summed
+    float2 acc = two(0.f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = (v * TPR + lane) * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f[v][e] = 0.f;
-      if (live && c < C) load_vec<VEC>(xr + c, f[v]);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s[0] += f[v][e];
+    for (int i = 0; i < PAIRS; ++i) acc = fadd2(acc, a.pair(i));
+    float s[1] = {acc.x + acc.y};
     group_sum<TPR>(s, red, turn);
     const float mean = s[0] * inv_c;
-    s[0] = 0.f;
+    acc = two(0.f);
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if ((v * TPR + lane) * VEC < C)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          f[v][e] -= mean;
-          s[0] += f[v][e] * f[v][e];
-        }
+    for (int i = 0; i < PAIRS; ++i) {
+      // columns past C (whole vectors, or single elements) stay out of the variance
+      float2 d = fsub2(a.pair(i), two(mean));
+      const int v = 2 * i / VEC;
+      if ((v * TPR + lane) * VEC >= C) d.x = 0.f;
+      if (((VEC == 1 ? v + 1 : v) * TPR + lane) * VEC >= C) d.y = 0.f;
+      acc = ffma2(d, d, acc);
+    }
+    s[0] = acc.x + acc.y;
     group_sum<TPR>(s, red, turn);
     const float rstd = 1.0f / sqrtf(s[0] * inv_c + eps);
     if (!live) continue;  // the loop's trip count is the block's, not the group's
@@ -147,12 +240,11 @@ __global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_fwd_kernel(long l
       mean_out[row] = mean;
       rstd_out[row] = rstd;
     }
-    T* yr = y + row * C;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (v * TPR + lane) * VEC;
       if (c >= C) continue;
-      float ww[VEC], bb[VEC];
+      float ww[VEC], bb[VEC], o[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         ww[e] = 1.f;
@@ -161,69 +253,37 @@ __global__ void __launch_bounds__(ln_threads<TPR>()) layernorm_fwd_kernel(long l
       if (w) load_vec<VEC>(w + c, ww);
       if (b) load_vec<VEC>(b + c, bb);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[v][e] = f[v][e] * rstd * ww[e] + bb[e];
-      store_vec<VEC>(yr + c, f[v]);
+      for (int e = 0; e < VEC; ++e) {
+        const float2 f = a.pair((v * VEC + e) / 2);
+        o[e] = fmaf((((v * VEC + e) & 1 ? f.y : f.x) - mean) * rstd, ww[e], bb[e]);
+      }
+      store_vec<VEC>(y + row * C + c, o);
     }
   }
 }
-
-// What one thread holds of a row before it is converted: 16 bytes, or one element.
-template <class T, int VEC>
-struct Raw {
-  uint4 r;
-  __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void clear() { r = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ float operator[](int e) const {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(w[e]);
-    } else {
-      const uint32_t h = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(h << 16);
-      return __half2float(__ushort_as_half(uint16_t(h)));
-    }
-  }
-};
-template <class T>
-struct Raw<T, 1> {
-  T r;
-  __device__ __forceinline__ void load(const T* p) { r = *p; }
-  __device__ __forceinline__ void clear() { r = from_f<T>(0.f); }
-  __device__ __forceinline__ float operator[](int) const { return to_f(r); }
-};
 
 // R rows per group and round; block i takes every gridDim.x-th round, and the
 // next round's rows are on their way while this one's are summed (they wait as
 // they lie in memory, so the second set costs few registers).  Partial sums of
 // the block's rows: part[(2 i) C ..] for dw, part[(2 i + 1) C ..] for db.
+// Columns past C hold dy = 0 and add nothing to any sum.
 template <class T, class W, int VEC, int TPR, int V, int R>
-__global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) layernorm_bwd_kernel(long long rows, int C,
-                                                                         const T* __restrict__ dy,
-                                                                         const T* __restrict__ x,
-                                                                         const W* __restrict__ w,
-                                                                         const float* __restrict__ mean_in,
-                                                                         const float* __restrict__ rstd_in,
-                                                                         T* __restrict__ dx, float* __restrict__ part) {
-  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR;
+__global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) layernorm_bwd_kernel(
+    long long rows, int C, const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
+    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part) {
+  constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR, PAIRS = V * VEC / 2;
   __shared__ float red[2 * 2 * R * THREADS / 32];
   extern __shared__ float cols[];  // [2][C], only with several groups
   pdl_launch();
   int turn = 0;
   const int g = threadIdx.x / TPR, lane = threadIdx.x % TPR;
   const float inv_c = 1.0f / float(C);
-  float ww[V][VEC], dw[V][VEC], db[V][VEC];
+  float2 ww[PAIRS], dw[PAIRS], db[PAIRS];
+  load_cols<W, VEC, TPR, V>(w, lane, C, 1.f, ww);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int c = (v * TPR + lane) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      ww[v][e] = 1.f;
-      dw[v][e] = db[v][e] = 0.f;
-    }
-    if (w && c < C) load_vec<VEC>(w + c, ww[v]);
-  }
+  for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = two(0.f);
   struct Rows {
-    Raw<T, VEC> x[R][V], d[R][V];
+    Row<T, VEC, TPR, V> x[R], d[R];
     float mean[R], rstd[R];
   };
   auto fetch = [&](Rows& a, long long row0) {
@@ -231,17 +291,8 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + g * R + r;
       const bool live = row < rows;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int c = (v * TPR + lane) * VEC;
-        if (live && c < C) {
-          a.x[r][v].load(x + row * C + c);
-          a.d[r][v].load(dy + row * C + c);
-        } else {
-          a.x[r][v].clear();
-          a.d[r][v].clear();
-        }
-      }
+      a.x[r].load(x + row * C, lane, C, live);
+      a.d[r].load(dy + row * C, lane, C, live);
       a.mean[r] = live ? mean_in[row] : 0.f;
       a.rstd[r] = live ? rstd_in[row] : 0.f;  // xhat = 0 in rows that are not there
     }
@@ -256,41 +307,38 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
     float sums[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      sums[2 * r] = sums[2 * r + 1] = 0.f;
+      const float2 rs = two(a.rstd[r]), mr = two(-a.mean[r] * a.rstd[r]);
+      float2 s1 = two(0.f), s2 = two(0.f);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if ((v * TPR + lane) * VEC >= C) continue;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float xh = (a.x[r][v][e] - a.mean[r]) * a.rstd[r], d = a.d[r][v][e];
-          const float gg = d * ww[v][e];
-          sums[2 * r] += gg;
-          sums[2 * r + 1] += gg * xh;
-          dw[v][e] += d * xh;
-          db[v][e] += d;
-        }
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 xh = ffma2(a.x[r].pair(i), rs, mr), d = a.d[r].pair(i), gg = fmul2(d, ww[i]);
+        s1 = fadd2(s1, gg);
+        s2 = ffma2(gg, xh, s2);
+        dw[i] = ffma2(d, xh, dw[i]);
+        db[i] = fadd2(db[i], d);
       }
+      sums[2 * r] = s1.x + s1.y;
+      sums[2 * r + 1] = s2.x + s2.y;
     }
     group_sum<TPR>(sums, red, turn);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + g * R + r;
       if (row >= rows) continue;
-      const float m1 = sums[2 * r] * inv_c, m2 = sums[2 * r + 1] * inv_c;
+      const float2 rs = two(a.rstd[r]), mr = two(-a.mean[r] * a.rstd[r]);
+      const float2 m1 = two(-sums[2 * r] * inv_c * a.rstd[r]), m2 = two(-sums[2 * r + 1] * inv_c * a.rstd[r]);
+      float2 o[PAIRS];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int c = (v * TPR + lane) * VEC;
-        if (c >= C) continue;
-        float o[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          o[e] = a.rstd[r] * (a.d[r][v][e] * ww[v][e] - m1 - (a.x[r][v][e] - a.mean[r]) * a.rstd[r] * m2);
-        store_vec<VEC>(dx + row * C + c, o);
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 xh = ffma2(a.x[r].pair(i), rs, mr);
+        o[i] = ffma2(fmul2(a.d[r].pair(i), ww[i]), rs, ffma2(xh, m2, m1));
       }
+      store_row<T, VEC, TPR, V>(dx + row * C, lane, C, o);
     }
     a = next;
   }
   if (!part) return;
+  auto at = [](const float2* f, int i) { return i & 1 ? f[i >> 1].y : f[i >> 1].x; };
   float* out = part + (long long)blockIdx.x * 2 * C;
   if (GROUPS > 1) {  // the groups' sums, added in their order
     for (int k = 0; k < GROUPS; ++k) {
@@ -301,8 +349,8 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
           if (c >= C) continue;
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            cols[c + e] = (k ? cols[c + e] : 0.f) + dw[v][e];
-            cols[C + c + e] = (k ? cols[C + c + e] : 0.f) + db[v][e];
+            cols[c + e] = (k ? cols[c + e] : 0.f) + at(dw, v * VEC + e);
+            cols[C + c + e] = (k ? cols[C + c + e] : 0.f) + at(db, v * VEC + e);
           }
         }
       __syncthreads();
@@ -315,8 +363,8 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
       if (c >= C) continue;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        out[c + e] = dw[v][e];
-        out[C + c + e] = db[v][e];
+        out[c + e] = at(dw, v * VEC + e);
+        out[C + c + e] = at(db, v * VEC + e);
       }
     }
   }
@@ -426,18 +474,19 @@ __global__ void __launch_bounds__(256) layernorm_part_long_kernel(long long rows
 struct LnShape {
   int vec, tpr, v;  // v = 0: the long-row kernels
 };
-// Forward: one warp per row while it holds it in 8 vectors a lane (32 single
-// elements), because then no barrier stands between the row's load and its store;
+// Forward: one warp per row while it holds it in 8 vectors a lane, because then no
+// barrier stands between the row's load and its store (65536 x 2048 bf16: 92 us
+// with one warp of 8 vectors a lane, 102 with two of 4, 117 with four of 2);
 // longer rows take more warps, and so do rows too few to give every SM a block.
 static LnShape ln_fwd_shape(long long rows, int C, int elem, bool aligned) {
   LnShape s;
   s.vec = aligned && C % (16 / elem) == 0 ? 16 / elem : 1;
-  const int units = (C + s.vec - 1) / s.vec, least = s.vec == 1 ? 8 : 1, most = s.vec == 1 ? 32 : 8;
+  const int units = (C + s.vec - 1) / s.vec, least = s.vec == 1 ? 8 : 1, most = 8;
   s.tpr = 32;
   while (s.tpr < 512 && s.tpr * most < units) s.tpr *= 2;
   s.v = least;
   while (s.tpr * s.v < units) s.v *= s.vec == 1 ? 4 : 2;
-  if (s.v > most) {
+  if (s.v > (s.vec == 1 ? 32 : 8)) {
     s.v = 0;
     return s;
   }
@@ -461,16 +510,19 @@ static LnShape ln_bwd_shape(int C, int elem, bool aligned) {
   return s;
 }
 constexpr int LN_LONG_PARTS = 64;
+constexpr int LN_MAX_PARTS = 2 * 160;  // partial rows of dw and db: one per block, two blocks an SM
 
 static int ln_bwd_blocks(long long rows, const LnShape& s, int rows_per_round) {
   const int threads = s.tpr > 256 ? s.tpr : 256, groups = threads / s.tpr;
   const long long rounds = (rows + (long long)groups * rows_per_round - 1) / ((long long)groups * rows_per_round);
-  return int(std::min<long long>(rounds, (long long)num_sms() * (threads > 256 ? 1 : 2)));
+  return int(std::min<long long>(rounds, std::min(num_sms() * (threads > 256 ? 1 : 2), LN_MAX_PARTS)));
 }
-// Rows per group and round; two rounds are in flight, 16 bytes of x and of dy per vector.
+// Rows per group and round; two rounds are in flight.  Four rows (half as many
+// barriers) spill at 128 registers: 177 against 155 us for 65536 x 2048 bf16, and
+// 226 against 151 us for 262144 x 512.
 template <int VEC, int V>
 constexpr int ln_rows() {
-  return VEC * V > 8 ? 1 : VEC == 1 ? 2 : 4;
+  return VEC * V > 8 ? 1 : 2;
 }
 
 template <class T, class W, int VEC, int TPR, int V>
@@ -558,7 +610,7 @@ static int layernorm_fwd(long long rows, int C, float eps, const void* x, const 
   return check_launch("layernorm_fwd_kernel");
 }
 
-static int ln_rows_of(const LnShape& s) { return s.vec * s.v > 8 ? 1 : s.vec == 1 ? 2 : 4; }
+static int ln_rows_of(const LnShape& s) { return s.vec * s.v > 8 ? 1 : 2; }
 
 template <class T, class W>
 static int layernorm_bwd(long long rows, int C, const void* dy, const void* x, const void* w, const float* mean,
@@ -625,8 +677,7 @@ static bool ln_vector(std::initializer_list<const void*> ps) {
 
 extern "C" size_t mea_layernorm_workspace_size(long long rows, int C) {
   if (rows < 0 || C <= 0) return 0;
-  // dw and db partials of at most two blocks an SM, on the largest part there is
-  return size_t(2) * size_t(C) * sizeof(float) * 2 * 160;
+  return size_t(2) * size_t(C) * sizeof(float) * mea::LN_MAX_PARTS;
 }
 
 extern "C" int mea_layernorm_forward(long long rows, int C, float eps, int dtype, int wdtype, const void* x, const void* w,
