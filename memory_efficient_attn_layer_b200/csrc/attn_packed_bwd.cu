@@ -884,7 +884,7 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   rc |= packed_map(&maps.dO, pd, d->dtype, dO, do_row, do_head, pd.Hq, pd.p, pd.tt);
   rc |= packed_map(&maps.k, pd, d->dtype, k, d->k_row, d->k_head, pd.Hkv, 1, 128);
   rc |= packed_map(&maps.v, pd, d->dtype, v, d->v_row, d->v_head, pd.Hkv, 1, 128);
-  if (rc) return set_error(MEA_ERR_CUDA, "packed attention backward: tensor map encode failed");
+  if (rc) return set_error(MEA_ERR_CUDA, "packed attention backward: tensor map encode failed (%d)", rc);
   PackedBwdParams p;
   p.d = pd;
   p.plan = packed_plan_view(pd, plan);

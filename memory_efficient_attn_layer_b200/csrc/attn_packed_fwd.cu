@@ -537,7 +537,7 @@ extern "C" int mea_packed_attention_forward(const mea_packed_dims* d, const void
   rc = packed_map(&maps.q, pd, d->dtype, q, d->q_row, d->q_head, pd.Hq, pd.p, pd.tt);
   rc |= packed_map(&maps.k, pd, d->dtype, k, d->k_row, d->k_head, pd.Hkv, 1, 128);
   rc |= packed_map(&maps.v, pd, d->dtype, v, d->v_row, d->v_head, pd.Hkv, 1, 128);
-  if (rc) return set_error(MEA_ERR_CUDA, "packed attention: tensor map encode failed");
+  if (rc) return set_error(MEA_ERR_CUDA, "packed attention: tensor map encode failed (%d)", rc);
   auto st = static_cast<cudaStream_t>(stream);
   if ((rc = run_packed_plan(pd, cu_seqlens, plan, status, st)) != MEA_OK) return rc;
   PackedFwdParams p;

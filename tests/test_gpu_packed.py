@@ -242,6 +242,26 @@ def test_other_stream_and_interleaved_calls():
             assert torch.equal(t, (want2 if i % 2 else want)[name])
 
 
+def test_calls_from_other_threads():
+    """The first CUDA call that a new thread makes: forward and backward (autograd's own thread) alike."""
+    import threading
+
+    q, k, v, do, cu = _make([300, 20], 4, 2, 64, BF, seed=30)
+    want, got = _run(q, k, v, do, cu), {}
+
+    def work(i):
+        got[i] = _run(q, k, v, do, cu)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 3
+    for x in got.values():
+        assert all(torch.equal(x[n], want[n]) for n in want)
+
+
 def test_captured_call_follows_the_lengths():
     """Forward and backward in a CUDA graph, replayed with other values and other lengths, two graphs in turn."""
     hq, hkv, n, total = 4, 2, 64, 400
