@@ -230,10 +230,11 @@ int mea_packed_attention_forward(const mea_packed_dims* d, const void* q, const 
                                  const int* cu_seqlens, void* o, float* lse2, void* plan, size_t plan_bytes,
                                  int* status, void* stream);
 /* dq, dk, dv of the same call from its o, lse2 and plan and from dO (strides
- * as q's).  delta: fp32 [total, Hq] workspace. */
+ * as q's).  delta: fp32 [total, Hq] workspace.  The plan's list stays, two
+ * counters in it are used: backward calls that overlap need plans of their own. */
 int mea_packed_attention_backward(const mea_packed_dims* d, const void* q, const void* k, const void* v, const void* o,
                                   const void* dO, long long do_row, long long do_head, const float* lse2,
-                                  const void* plan, size_t plan_bytes, float* delta, void* dq, void* dk, void* dv,
+                                  void* plan, size_t plan_bytes, float* delta, void* dq, void* dk, void* dv,
                                   int* status, void* stream);
 
 /* ---------------------------------------------------------------- no allocation

@@ -19,13 +19,17 @@
 namespace mea {
 
 // ---- work plan (device memory, written by packed_plan_kernel) ----
-// header, then int4 items {first row of the sequence, its length, tile, 0}:
-// query tiles (cap_q) and 128-row key tiles (cap_k), each sorted by falling
-// work so that the tiles that take longest start first.
+// header, then int4 entries, one per tile: query tiles (cap_q) and 128-row key
+// tiles (cap_k).  An entry is {first row of the sequence, its length, z, by_tile}.
+// Tile number idx of the whole list belongs to entry idx / heads.  by_tile = 1:
+// the entry is tile z and the head idx % heads.  by_tile = 0: z tiles are listed
+// before the sequence's own nt entries, and there idx - z * heads = head * nt + n
+// for the n-th tile from the one that takes longest.
 struct PackedHeader {
-  int n_q, n_k;    // items of each kind
-  int first, end;  // rows [first, end) belong to sequences
-  int pad[4];
+  int n_q, n_k;        // entries of each kind
+  int first, end;      // rows [first, end) belong to sequences
+  int next_q, next_k;  // the backward's next tiles
+  int pad[2];
 };
 
 struct PackedDims {
@@ -87,6 +91,27 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int r0, int lane) {
   for (int c = 0; c < HD / 64; ++c)
     for (int u = lane; u < units; u += 32) sts128(tile + c * 16384 + r0 * 128 + u * 16, 0, 0, 0, 0);
 }
+
+// Where tile idx of a list lies: sequence, head (group) and the tile in it.
+// LAST_FIRST: a sequence's last tile takes longest (query tiles), else its first.
+template <bool LAST_FIRST>
+struct PackedTile {
+  int seq0, len, head, tile;
+  __device__ __forceinline__ PackedTile(const int4* items, int idx, int heads, int rows) {
+    const int i = idx / heads;
+    const int4 e = items[i];
+    seq0 = e.x;
+    len = e.y;
+    head = idx - i * heads;
+    tile = e.z;
+    if (!e.w) {
+      const int nt = (len + rows - 1) / rows, off = idx - e.z * heads;
+      head = off / nt;
+      tile = off - head * nt;
+      if (LAST_FIRST) tile = nt - 1 - tile;
+    }
+  }
+};
 
 // Rows of `width` 16-byte units outside [first, end) of a [total, width] output
 // to zero, spread over the grid: no sequence owns them.

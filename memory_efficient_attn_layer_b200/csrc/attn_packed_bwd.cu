@@ -35,6 +35,7 @@ struct PackedBwdParams {
   uint16_t* dq;        // [total, Hq, N]
   uint16_t* dk;        // [total, Hkv, N]
   uint16_t* dv;
+  int *next_q, *next_k;  // counters in the plan
   int* status;
 };
 struct PackedBwdMaps {
@@ -43,13 +44,15 @@ struct PackedBwdMaps {
 
 // ---------------------------------------------------------------- delta
 // 16 lanes per (token, head) row, 16 bytes of O and dO each, four rows in
-// flight; also clears the rows of dQ, dK and dV that no sequence owns.
+// flight; also clears the rows of dQ, dK and dV that no sequence owns, and the
+// counters that the next two kernels draw their tiles from.
 constexpr int DELTA_ROWS = 64;  // rows per 256-thread block
 template <class T>
-__global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, const PackedHeader* head, const uint16_t* o,
+__global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, PackedHeader* head, const uint16_t* o,
                                                            const uint16_t* dO, long long do_row, long long do_head,
                                                            float* delta, uint4* dq, uint4* dk, uint4* dv) {
   pdl_launch();
+  if (blockIdx.x == 0 && threadIdx.x == 0) head->next_q = head->next_k = 0;
   const long long rows = (long long)d.total * d.Hq;
   const int sub = threadIdx.x & 15;
   const long long r0 = (long long)blockIdx.x * DELTA_ROWS + (threadIdx.x >> 4);
@@ -83,17 +86,32 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, const P
 }
 
 // ---------------------------------------------------------------- common
-// Items of a persistent CTA over a list sorted by falling work: rounds of
-// gridDim.x items, every second one in reverse, so no CTA draws the longest of
-// each round.
-struct SnakeItems {
-  int n, round;
-  __device__ explicit SnakeItems(int n_) : n(n_), round(0) {}
-  __device__ int index() const {
-    return round * int(gridDim.x) + ((round & 1) ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
+// Tiles of a persistent CTA: warp 0 draws the next number from a counter in the
+// plan (long tiles first, so the CTAs end together) and hands it to the other
+// roles through a ring of four slots; each reader copies the number and gives the
+// slot back.  Which CTA takes a tile changes no result.
+struct Feed {
+  static constexpr int SLOTS = 4;
+  uint32_t full, empty;  // mbarriers, SLOTS each
+  volatile int* idx;
+  __device__ void put(int n, int value, Guard& g) const {  // one thread
+    if (!mbar_wait(empty + 8u * (n % SLOTS), ((n / SLOTS) & 1) ^ 1, g, 30)) return;
+    idx[n % SLOTS] = value;
+    mbar_arrive(full + 8u * (n % SLOTS));
   }
-  // False once no later round can hold an item either (a reversed last round may skip this CTA).
-  __device__ bool done() const { return round * (long long)gridDim.x >= n; }
+  __device__ int get(int n, Guard& g) const {  // one thread; -1: no more tiles
+    if (!mbar_wait(full + 8u * (n % SLOTS), (n / SLOTS) & 1, g, 31)) return -1;
+    const int v = idx[n % SLOTS];
+    mbar_arrive(empty + 8u * (n % SLOTS));
+    return v;
+  }
+  __device__ int get_warp(int n, Guard& g, int lane) const {  // a whole warp
+    int v = -1;
+    if (lane == 0) v = get(n, g);
+    v = __shfl_sync(0xffffffffu, v, 0);
+    g.ok = __shfl_sync(0xffffffffu, int(g.ok), 0) && g.ok;
+    return v;
+  }
 };
 
 // 32 columns of this thread's TMEM lane times `scale` to 16-bit values at out[c], c < n_left.
@@ -121,20 +139,20 @@ struct PackedDqCfg {
   static constexpr uint32_t S_COL = 0, DP_COL = 128, DS_COL = 256, DQ_COL = 320;
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
-  static constexpr size_t SMEM = 1024 + OFF_BAR + 256;
+  static constexpr size_t SMEM = 1024 + OFF_BAR + 512;
 };
 
 struct DqItem {
   int seq0, len, t0, t1, nkv, h0, kvh;
+  __device__ DqItem() {}
   __device__ DqItem(const PackedDims& d, const PackedPlan& plan, int idx) {
-    const int i = idx / d.hg;
-    const int4 it = plan.q_items[i];
-    seq0 = it.x;
-    len = it.y;
-    t0 = it.z * d.tt;
+    const PackedTile<true> it(plan.q_items, idx, d.hg, d.tt);
+    seq0 = it.seq0;
+    len = it.len;
+    t0 = it.tile * d.tt;
     t1 = min(t0 + d.tt, len);
     nkv = (t1 + 127) >> 7;
-    h0 = (idx - i * d.hg) * d.p;
+    h0 = it.head * d.p;
     kvh = h0 / (d.Hq / d.Hkv);
   }
 };
@@ -169,7 +187,8 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
   const uint32_t ds_full = b0 + 8u * 16, ds_free = b0 + 8u * 17;   // dS written / read by the dQ MMAs
   const uint32_t dq_full = b0 + 8u * 18, dq_empty = b0 + 8u * 19;  // an item's dQ complete / read out
   const uint32_t k_raw = b0 + 8u * 20, drain_bar = b0 + 8u * 21;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
+  const Feed feed{b0 + 8u * 22, b0 + 8u * 26, reinterpret_cast<int*>(bars + 31)};
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -185,6 +204,10 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     mbar_init(dq_empty, 256);
     mbar_init(k_raw, 1);
     mbar_init(drain_bar, 1);
+    for (int i = 0; i < Feed::SLOTS; ++i) {
+      mbar_init(feed.full + 8u * i, 1);
+      mbar_init(feed.empty + 8u * i, 9);  // MMA, eight softmax warps
+    }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -207,9 +230,15 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     for (int s = 0; s < KS; ++s) kpar[s] = -1;
     for (int s = 0; s < VS; ++s) vpar[s] = -1;
     int n = 0, item = 0, raw = 0;
-    for (SnakeItems it(n_items); !it.done() && g.ok; ++it.round) {
-      if (it.index() >= n_items) continue;
-      const DqItem w(p.d, p.plan, it.index());
+    int idx = blockIdx.x;  // the grid holds no more CTAs than there can be tiles
+    while (g.ok) {
+      int after = 0;
+      if (lead) {
+        feed.put(item, idx < n_items ? idx : -1, g);
+        if (idx < n_items) after = int(gridDim.x) + atomicAdd(p.next_q, 1);
+      }
+      if (idx >= n_items) break;
+      const DqItem w(p.d, p.plan, idx);
       const int qb = item % QB;
       if (lead && (item < QB || mbar_wait(q_empty(qb), uint32_t((item / QB - 1) & 1), g, 1))) {
         mbar_expect_tx(q_full(qb), 2u * uint32_t(p.d.p * p.d.tt) * 128 * Tile::NCHUNK);
@@ -256,6 +285,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           if (lead) mbar_arrive(k_full(sk));
         }
       }
+      idx = __shfl_sync(0xffffffffu, after, 0);
     }
     if (lead) {
       if (!g.ok) {
@@ -281,11 +311,10 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     if (elect_one()) {
       bool any = false;
       // S and dP run one step ahead of dQ, across items: (n1, item1, j1) is their next step.
-      int n1 = 0, item1 = 0, j1 = 0, nkv1 = 0;
-      SnakeItems it1(n_items);
-      auto settle = [&]() {  // it1 at its next item, or done
-        while (!it1.done() && it1.index() >= n_items) ++it1.round;
-        if (!it1.done()) nkv1 = DqItem(p.d, p.plan, it1.index()).nkv;
+      int n1 = 0, item1 = 0, j1 = 0, nkv1 = 0;  // nkv1 = 0: no more items
+      auto settle = [&]() {
+        const int idx = feed.get(item1, g);
+        nkv1 = idx < 0 ? 0 : DqItem(p.d, p.plan, idx).nkv;
       };
       settle();
       auto issue_s = [&]() -> bool {
@@ -316,19 +345,18 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
         if (++j1 == nkv1) {
           j1 = 0;
           ++item1;
-          ++it1.round;
           settle();
         }
         return true;
       };
-      int n = 0, item = 0;
-      if (!it1.done() && issue_s()) issue_dp();
-      for (SnakeItems it(n_items); !it.done() && g.ok; ++it.round) {
-        if (it.index() >= n_items) continue;
-        const int nkv = DqItem(p.d, p.plan, it.index()).nkv;
+      int n = 0, item = 0, nkv = nkv1;
+      if (nkv && issue_s()) issue_dp();
+      while (nkv && g.ok) {
+        int nkv_next = 0;
         for (int j = 0; j < nkv; ++j, ++n) {
           const int sk = n % KS;
-          const bool more = !it1.done();
+          const bool more = nkv1 > 0;
+          if (j + 1 == nkv) nkv_next = nkv1;  // the lookahead stands at the next item by now
           // With one Q/dO buffer the next item's rows arrive late: this item's last dQ goes first.
           const bool late = QB == 1 && j + 1 == nkv;
           auto ahead = [&]() -> bool {
@@ -347,6 +375,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           if (j + 1 == nkv) mma_commit(dq_full);
           if (more && late && !ahead()) break;
         }
+        nkv = nkv_next;
         ++item;
       }
       if (!g.ok && any) {
@@ -363,9 +392,11 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     const int tok = r / p.d.p, hr = r - tok * p.d.p;
     bool ok = true;
     int n = 0, item = 0;
-    for (SnakeItems it(n_items); !it.done() && ok; ++it.round) {
-      if (it.index() >= n_items) continue;
-      const DqItem w(p.d, p.plan, it.index());
+    while (ok) {
+      const int idx = feed.get_warp(item, g, lane);
+      ok = g.ok;
+      if (!ok || idx < 0) break;
+      const DqItem w(p.d, p.plan, idx);
       const int t = w.t0 + tok;
       const bool live = r < p.d.p * p.d.tt && t < w.t1;
       const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
@@ -450,18 +481,18 @@ struct PackedDkvCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static_assert(DK_COL + HD <= 512, "TMEM budget");
   static constexpr uint32_t OFF_Q = KVB * 2 * TB, OFF_ROW = OFF_Q + ST * 2 * TB, OFF_BAR = OFF_ROW + ST * 1024;
-  static constexpr size_t SMEM = 1024 + OFF_BAR + 256;
+  static constexpr size_t SMEM = 1024 + OFF_BAR + 512;
 };
 
 struct DkvItem {
   int seq0, len, k0, kvh, qt0, nqt, groups, h0;
+  __device__ DkvItem() {}
   __device__ DkvItem(const PackedDims& d, const PackedPlan& plan, int idx) {
-    const int i = idx / d.Hkv;
-    const int4 it = plan.k_items[i];
-    kvh = idx - i * d.Hkv;
-    seq0 = it.x;
-    len = it.y;
-    k0 = it.z * 128;
+    const PackedTile<false> it(plan.k_items, idx, d.Hkv, 128);
+    kvh = it.head;
+    seq0 = it.seq0;
+    len = it.len;
+    k0 = it.tile * 128;
     qt0 = k0 / d.tt;
     nqt = (len + d.tt - 1) / d.tt;
     const int G = d.Hq / d.Hkv;
@@ -503,7 +534,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   const uint32_t dp_full = b0 + 8u * 20, ds_full = b0 + 8u * 21;  // dP^T computed / dS^T written over it
   const uint32_t acc_full = b0 + 8u * 22, acc_empty = b0 + 8u * 23;  // an item's dK, dV complete / read out
   const uint32_t raw_bar = b0 + 8u * 24, drain_bar = b0 + 8u * 25;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
+  const Feed feed{b0 + 8u * 26, b0 + 8u * 30, reinterpret_cast<int*>(bars + 35)};
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -520,6 +552,10 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     mbar_init(acc_empty, 256);
     mbar_init(raw_bar, 1);
     mbar_init(drain_bar, 1);
+    for (int i = 0; i < Feed::SLOTS; ++i) {
+      mbar_init(feed.full + 8u * i, 1);
+      mbar_init(feed.empty + 8u * i, 10);  // MMA, warp 2, eight softmax warps
+    }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -549,9 +585,15 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     int kvpar[2] = {-1, -1}, qpar[ST];
     for (int s = 0; s < ST; ++s) qpar[s] = -1;
     int n = 0, item = 0, raw = 0;
-    for (SnakeItems it(n_items); !it.done() && g.ok; ++it.round) {
-      if (it.index() >= n_items) continue;
-      const DkvItem w(p.d, p.plan, it.index());
+    int idx = blockIdx.x;  // the grid holds no more CTAs than there can be tiles
+    while (g.ok) {
+      int after = 0;
+      if (lead) {
+        feed.put(item, idx < n_items ? idx : -1, g);
+        if (idx < n_items) after = int(gridDim.x) + atomicAdd(p.next_k, 1);
+      }
+      if (idx >= n_items) break;
+      const DkvItem w(p.d, p.plan, idx);
       const int kb = item % KVB;
       if (lead && (item < KVB || mbar_wait(kv_empty(kb), uint32_t((item / KVB - 1) & 1), g, 1))) {
         mbar_expect_tx(kv_full(kb), 2 * TB);
@@ -595,6 +637,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             if (lead) mbar_arrive(qdo_full(s));
           }
         }
+      idx = __shfl_sync(0xffffffffu, after, 0);
     }
     if (lead) {
       if (!g.ok) {
@@ -615,25 +658,29 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     if (elect_one()) {
       bool any = false;
       // S^T and dP^T run ahead of dV and dK, across items: their next steps.
-      struct Ahead {
-        SnakeItems it;
-        int n, item, left;
+      // With two S^T buffers S^T may be an item ahead of dP^T, so the steps of up to
+      // three items in a row are kept (0: no more).
+      int item_steps[3], got = 0;
+      auto steps_of = [&](int item) -> int {
+        while (got <= item) {
+          const int idx = feed.get(got, g);
+          const int st = idx < 0 ? 0 : DkvItem(p.d, p.plan, idx).steps();
+          if (got % 3 == 0) item_steps[0] = st;
+          if (got % 3 == 1) item_steps[1] = st;
+          if (got % 3 == 2) item_steps[2] = st;
+          ++got;
+          if (st == 0) break;
+        }
+        return item % 3 == 0 ? item_steps[0] : item % 3 == 1 ? item_steps[1] : item_steps[2];
       };
-      auto settle = [&](Ahead& a) {
-        while (!a.it.done() && a.it.index() >= n_items) ++a.it.round;
-        if (!a.it.done()) a.left = DkvItem(p.d, p.plan, a.it.index()).steps();
+      struct Ahead {
+        int n, item, left;  // left = 0: no more steps
       };
       auto advance = [&](Ahead& a) {
         ++a.n;
-        if (--a.left == 0) {
-          ++a.item;
-          ++a.it.round;
-          settle(a);
-        }
+        if (--a.left == 0) a.left = steps_of(++a.item);
       };
-      Ahead as{SnakeItems(n_items), 0, 0, 0}, ad{SnakeItems(n_items), 0, 0, 0};
-      settle(as);
-      settle(ad);
+      Ahead as{0, 0, steps_of(0)}, ad = as;
       auto issue_s = [&]() -> bool {  // S^T = K Q^T
         const int kb = as.item % KVB, s = as.n % ST;
         if (!mbar_wait(kv_full(kb), (as.item / KVB) & 1, g, 6)) return false;
@@ -659,15 +706,13 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
         advance(ad);
       };
       int n = 0, item = 0;
-      if (!as.it.done() && issue_s()) issue_dp();
-      for (SnakeItems it(n_items); !it.done() && g.ok; ++it.round) {
-        if (it.index() >= n_items) continue;
-        const int steps = DkvItem(p.d, p.plan, it.index()).steps();
+      if (as.left && issue_s()) issue_dp();
+      for (int steps = steps_of(0); steps && g.ok; steps = steps_of(++item)) {
         for (int k = 0; k < steps; ++k, ++n) {
           const int s = n % ST;
           const uint32_t pt = tmem + Cfg::S_COL + 128 * (n % SB), dst = tmem + Cfg::DP_COL;
           // Two S^T buffers: the next one is free once dV of the step before has been issued.
-          if (SB == 2 && !as.it.done() && !issue_s()) break;
+          if (SB == 2 && as.left && !issue_s()) break;
           if (!mbar_wait(p_full(n % SB), (n / SB) & 1, g, 8)) break;
           if (k == 0 && item > 0 && !mbar_wait(acc_empty, (item - 1) & 1, g, 9)) break;
           tc_fence_after();
@@ -676,7 +721,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           for (int kc = 0; kc < 8; ++kc)
             mma_ts(tmem + Cfg::DV_COL, pt + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sdO(s), 128, kc), IDESC_KV,
                    (k > 0 || kc > 0) ? 1u : 0u);
-          if (SB == 1 && !as.it.done() && !issue_s()) break;
+          if (SB == 1 && as.left && !issue_s()) break;
           if (!mbar_wait(ds_full, n & 1, g, 10)) break;
           tc_fence_after();
           // dK += dS^T Q
@@ -686,9 +731,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
                    (k > 0 || kc > 0) ? 1u : 0u);
           mma_commit(qdo_empty(s));
           if (k + 1 == steps) mma_commit(acc_full);
-          if (!ad.it.done()) issue_dp();
+          if (ad.left) issue_dp();
         }
-        ++item;
       }
       if (!g.ok && any) {
         mma_commit(drain_bar);
@@ -698,9 +742,10 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   } else if (warp == 2) {
     // ---------------- -lse2 and delta of each step's 128 query rows ----------------
     int n = 0;
-    for (SnakeItems it(n_items); !it.done() && g.ok; ++it.round) {
-      if (it.index() >= n_items) continue;
-      const DkvItem w(p.d, p.plan, it.index());
+    for (int item = 0; g.ok; ++item) {
+      const int idx = feed.get_warp(item, g, lane);
+      if (!g.ok || idx < 0) break;
+      const DkvItem w(p.d, p.plan, idx);
       for (int gi = 0; gi < w.groups && g.ok; ++gi)
         for (int qt = w.qt0; qt < w.nqt; ++qt, ++n) {
           const int s = n % ST;
@@ -726,9 +771,11 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     int n = 0, item = 0;
-    for (SnakeItems it(n_items); !it.done() && ok; ++it.round) {
-      if (it.index() >= n_items) continue;
-      const DkvItem w(p.d, p.plan, it.index());
+    while (ok) {
+      const int idx = feed.get_warp(item, g, lane);
+      ok = g.ok;
+      if (!ok || idx < 0) break;
+      const DkvItem w(p.d, p.plan, idx);
       const int key = w.k0 + r;
       for (int gi = 0; gi < w.groups && ok; ++gi)
         for (int qt = w.qt0; qt < w.nqt; ++qt, ++n) {
@@ -847,7 +894,7 @@ static int launch_packed_bwd(const PackedBwdMaps& maps, const PackedBwdParams& p
 
 extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const void* q, const void* k, const void* v,
                                              const void* o, const void* dO, long long do_row, long long do_head,
-                                             const float* lse2, const void* plan, size_t plan_bytes, float* delta,
+                                             const float* lse2, void* plan, size_t plan_bytes, float* delta,
                                              void* dq, void* dk, void* dv, int* status, void* stream) {
   using namespace mea;
   PackedDims pd;
@@ -895,13 +942,16 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
+  PackedHeader* head = const_cast<PackedHeader*>(p.plan.head);
+  p.next_q = &head->next_q;
+  p.next_k = &head->next_k;
   p.status = status;
   const long long rows = (long long)pd.total * pd.Hq, blocks = (rows + DELTA_ROWS - 1) / DELTA_ROWS;
   if (blocks > 0x7fffffffLL)
     return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention backward: %d rows x %d heads are too many", pd.total, pd.Hq);
   const bool bf = d->dtype == MEA_BF16;
   (bf ? packed_delta_kernel<Bf16> : packed_delta_kernel<Fp16>)<<<unsigned(blocks), 256, 0, st>>>(
-      pd, p.plan.head, static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dO), do_row, do_head, delta,
+      pd, head, static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dO), do_row, do_head, delta,
       static_cast<uint4*>(dq), static_cast<uint4*>(dk), static_cast<uint4*>(dv));
   if ((rc = check_launch("packed_delta_kernel")) != MEA_OK) return rc;
   if (bf) return pd.N <= 64 ? launch_packed_bwd<64, Bf16>(maps, p, st) : launch_packed_bwd<128, Bf16>(maps, p, st);

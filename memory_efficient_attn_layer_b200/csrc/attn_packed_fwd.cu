@@ -207,13 +207,12 @@ __global__ void __launch_bounds__(192, 2) packed_fwd_kernel(const __grid_constan
   const PackedHeader hd = *p.plan.head;
   zero_outside(static_cast<uint4*>(p.o), p.d.total, hd.first, hd.end, (long long)p.d.Hq * p.d.N / 8, blockIdx.x,
                gridDim.x, threadIdx.x, blockDim.x);
-  const int idx = int(blockIdx.x) / p.d.hg;
-  if (idx >= hd.n_q) return;
-  const int4 item = p.plan.q_items[idx];
-  const int h0 = (int(blockIdx.x) - idx * p.d.hg) * p.d.p;  // first head
+  if (int(blockIdx.x) / p.d.hg >= hd.n_q) return;
+  const PackedTile<true> item(p.plan.q_items, blockIdx.x, p.d.hg, p.d.tt);
+  const int h0 = item.head * p.d.p;  // first head
   const int kvh = h0 / (p.d.Hq / p.d.Hkv);
-  const int seq0 = item.x, len = item.y;
-  const int t0 = item.z * p.d.tt;
+  const int seq0 = item.seq0, len = item.len;
+  const int t0 = item.tile * p.d.tt;
   const int t1 = min(t0 + p.d.tt, len);
   const int nkv = (t1 + 127) >> 7;
 
