@@ -19,30 +19,33 @@
 namespace mea {
 
 // ---- work plan (device memory, written by packed_plan_kernel) ----
-// header, then int4 entries, one per tile: query tiles (cap_q) and 128-row key
-// tiles (cap_k).  An entry is {first row of the sequence, its length, z, by_tile}.
+// header, then three lists of int4 entries, one per tile: query tiles (the dQ
+// kernel's), 128-row key tiles, and the forward's items of one or two query
+// tiles.  An entry is {first row of the sequence, its length, z, by_tile}.
 // Tile number idx of the whole list belongs to entry idx / heads.  by_tile = 1:
 // the entry is tile z and the head idx % heads.  by_tile = 0: z tiles are listed
 // before the sequence's own nt entries, and there idx - z * heads = head * nt + n
 // for the n-th tile from the one that takes longest.
 struct PackedHeader {
-  int n_q, n_k;        // entries of each kind
-  int first, end;      // rows [first, end) belong to sequences
-  int next_q, next_k;  // the backward's next tiles
-  int pad[2];
+  int n[3];        // entries of each list
+  int first, end;  // rows [first, end) belong to sequences
+  int next[3];     // next tile to be drawn from each list
 };
 
 struct PackedDims {
   int total, n_seqs, Hq, Hkv, N;
   int p, tt;        // heads and tokens of a query tile
-  int cap_q, cap_k;
   int hg;           // query tiles per token tile: Hq / p
+  int streams;      // query tiles of a forward item
+  int rows[3];      // tokens of a tile of each list
+  int heads[3];     // tiles per entry: head groups, or key/value heads
+  int cap[3];       // entries there can be
 };
 
+enum PackedList { LIST_Q = 0, LIST_K = 1, LIST_FWD = 2 };
 struct PackedPlan {
-  const PackedHeader* head;
-  const int4* q_items;
-  const int4* k_items;
+  PackedHeader* head;
+  int4* list[3];
 };
 
 // ---- element types ----
@@ -91,6 +94,34 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int r0, int lane) {
   for (int c = 0; c < HD / 64; ++c)
     for (int u = lane; u < units; u += 32) sts128(tile + c * 16384 + r0 * 128 + u * 16, 0, 0, 0, 0);
 }
+
+// Tiles of a persistent CTA: warp 0 draws the next number from a counter in the
+// plan (long tiles first, so the CTAs end together) and hands it to the other
+// roles through a ring of four slots; each reader copies the number and gives the
+// slot back.  Which CTA takes a tile changes no result.
+struct Feed {
+  static constexpr int SLOTS = 4;
+  uint32_t full, empty;  // mbarriers, SLOTS each
+  volatile int* idx;
+  __device__ void put(int n, int value, Guard& g) const {  // one thread
+    if (!mbar_wait(empty + 8u * (n % SLOTS), ((n / SLOTS) & 1) ^ 1, g, 30)) return;
+    idx[n % SLOTS] = value;
+    mbar_arrive(full + 8u * (n % SLOTS));
+  }
+  __device__ int get(int n, Guard& g) const {  // one thread; -1: no more tiles
+    if (!mbar_wait(full + 8u * (n % SLOTS), (n / SLOTS) & 1, g, 31)) return -1;
+    const int v = idx[n % SLOTS];
+    mbar_arrive(empty + 8u * (n % SLOTS));
+    return v;
+  }
+  __device__ int get_warp(int n, Guard& g, int lane) const {  // a whole warp
+    int v = -1;
+    if (lane == 0) v = get(n, g);
+    v = __shfl_sync(0xffffffffu, v, 0);
+    g.ok = __shfl_sync(0xffffffffu, int(g.ok), 0) && g.ok;
+    return v;
+  }
+};
 
 // Where tile idx of a list lies: sequence, head (group) and the tile in it.
 // LAST_FIRST: a sequence's last tile takes longest (query tiles), else its first.

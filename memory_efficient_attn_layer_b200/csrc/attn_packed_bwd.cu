@@ -35,7 +35,6 @@ struct PackedBwdParams {
   uint16_t* dq;        // [total, Hq, N]
   uint16_t* dk;        // [total, Hkv, N]
   uint16_t* dv;
-  int *next_q, *next_k;  // counters in the plan
   int* status;
 };
 struct PackedBwdMaps {
@@ -52,7 +51,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, PackedH
                                                            const uint16_t* dO, long long do_row, long long do_head,
                                                            float* delta, uint4* dq, uint4* dk, uint4* dv) {
   pdl_launch();
-  if (blockIdx.x == 0 && threadIdx.x == 0) head->next_q = head->next_k = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) head->next[LIST_Q] = head->next[LIST_K] = 0;
   const long long rows = (long long)d.total * d.Hq;
   const int sub = threadIdx.x & 15;
   const long long r0 = (long long)blockIdx.x * DELTA_ROWS + (threadIdx.x >> 4);
@@ -86,34 +85,6 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, PackedH
 }
 
 // ---------------------------------------------------------------- common
-// Tiles of a persistent CTA: warp 0 draws the next number from a counter in the
-// plan (long tiles first, so the CTAs end together) and hands it to the other
-// roles through a ring of four slots; each reader copies the number and gives the
-// slot back.  Which CTA takes a tile changes no result.
-struct Feed {
-  static constexpr int SLOTS = 4;
-  uint32_t full, empty;  // mbarriers, SLOTS each
-  volatile int* idx;
-  __device__ void put(int n, int value, Guard& g) const {  // one thread
-    if (!mbar_wait(empty + 8u * (n % SLOTS), ((n / SLOTS) & 1) ^ 1, g, 30)) return;
-    idx[n % SLOTS] = value;
-    mbar_arrive(full + 8u * (n % SLOTS));
-  }
-  __device__ int get(int n, Guard& g) const {  // one thread; -1: no more tiles
-    if (!mbar_wait(full + 8u * (n % SLOTS), (n / SLOTS) & 1, g, 31)) return -1;
-    const int v = idx[n % SLOTS];
-    mbar_arrive(empty + 8u * (n % SLOTS));
-    return v;
-  }
-  __device__ int get_warp(int n, Guard& g, int lane) const {  // a whole warp
-    int v = -1;
-    if (lane == 0) v = get(n, g);
-    v = __shfl_sync(0xffffffffu, v, 0);
-    g.ok = __shfl_sync(0xffffffffu, int(g.ok), 0) && g.ok;
-    return v;
-  }
-};
-
 // 32 columns of this thread's TMEM lane times `scale` to 16-bit values at out[c], c < n_left.
 template <class T>
 __device__ __forceinline__ void store_cols32(uint32_t taddr, float scale, uint16_t* out, int n_left, bool live) {
@@ -146,7 +117,7 @@ struct DqItem {
   int seq0, len, t0, t1, nkv, h0, kvh;
   __device__ DqItem() {}
   __device__ DqItem(const PackedDims& d, const PackedPlan& plan, int idx) {
-    const PackedTile<true> it(plan.q_items, idx, d.hg, d.tt);
+    const PackedTile<true> it(plan.list[LIST_Q], idx, d.hg, d.tt);
     seq0 = it.seq0;
     len = it.len;
     t0 = it.tile * d.tt;
@@ -220,7 +191,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_launch();
-  const int n_items = p.plan.head->n_q * p.d.hg;
+  const int n_items = p.plan.head->n[LIST_Q] * p.d.hg;
   Guard g(p.status, KID_PACKED_DQ);
 
   if (warp == 0) {
@@ -235,7 +206,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
       int after = 0;
       if (lead) {
         feed.put(item, idx < n_items ? idx : -1, g);
-        if (idx < n_items) after = int(gridDim.x) + atomicAdd(p.next_q, 1);
+        if (idx < n_items) after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_Q], 1);
       }
       if (idx >= n_items) break;
       const DqItem w(p.d, p.plan, idx);
@@ -488,7 +459,7 @@ struct DkvItem {
   int seq0, len, k0, kvh, qt0, nqt, groups, h0;
   __device__ DkvItem() {}
   __device__ DkvItem(const PackedDims& d, const PackedPlan& plan, int idx) {
-    const PackedTile<false> it(plan.k_items, idx, d.Hkv, 128);
+    const PackedTile<false> it(plan.list[LIST_K], idx, d.Hkv, 128);
     kvh = it.head;
     seq0 = it.seq0;
     len = it.len;
@@ -575,7 +546,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
-  const int n_items = p.plan.head->n_k * p.d.Hkv;
+  const int n_items = p.plan.head->n[LIST_K] * p.d.Hkv;
   Guard g(p.status, KID_PACKED_DKV);
 
   if (warp == 0) {
@@ -590,7 +561,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       int after = 0;
       if (lead) {
         feed.put(item, idx < n_items ? idx : -1, g);
-        if (idx < n_items) after = int(gridDim.x) + atomicAdd(p.next_k, 1);
+        if (idx < n_items) after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
       }
       if (idx >= n_items) break;
       const DkvItem w(p.d, p.plan, idx);
@@ -880,7 +851,7 @@ static int launch_packed_bwd(const PackedBwdMaps& maps, const PackedBwdParams& p
     return set_error(MEA_ERR_CUDA, "cudaFuncSetAttribute(packed backward) failed");
   const int sms = num_sms();
   cudaLaunchAttribute attr;
-  const long long nq = (long long)p.d.cap_q * p.d.hg, nk = (long long)p.d.cap_k * p.d.Hkv;
+  const long long nq = (long long)p.d.cap[LIST_Q] * p.d.hg, nk = (long long)p.d.cap[LIST_K] * p.d.Hkv;
   cudaLaunchConfig_t cfg = packed_launch(int(nq < sms ? nq : sms), 384, PackedDqCfg<HD>::SMEM, st, &attr);
   cudaLaunchKernelEx(&cfg, dq, maps, p);
   int rc = check_launch("packed_dq_kernel");
@@ -942,16 +913,13 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
-  PackedHeader* head = const_cast<PackedHeader*>(p.plan.head);
-  p.next_q = &head->next_q;
-  p.next_k = &head->next_k;
   p.status = status;
   const long long rows = (long long)pd.total * pd.Hq, blocks = (rows + DELTA_ROWS - 1) / DELTA_ROWS;
   if (blocks > 0x7fffffffLL)
     return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention backward: %d rows x %d heads are too many", pd.total, pd.Hq);
   const bool bf = d->dtype == MEA_BF16;
   (bf ? packed_delta_kernel<Bf16> : packed_delta_kernel<Fp16>)<<<unsigned(blocks), 256, 0, st>>>(
-      pd, head, static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dO), do_row, do_head, delta,
+      pd, p.plan.head, static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dO), do_row, do_head, delta,
       static_cast<uint4*>(dq), static_cast<uint4*>(dk), static_cast<uint4*>(dv));
   if ((rc = check_launch("packed_delta_kernel")) != MEA_OK) return rc;
   if (bf) return pd.N <= 64 ? launch_packed_bwd<64, Bf16>(maps, p, st) : launch_packed_bwd<128, Bf16>(maps, p, st);

@@ -4,18 +4,23 @@
 // within each sequence, in one pass over its keys with the running row maximum
 // and sum.  lse2 = max + log2(sum) per row (log2 units) is kept for the backward.
 //
-// One CTA = one query tile of the plan (tt tokens x p heads, 128 rows), two
-// CTAs per SM, so one CTA's MMAs run under the other's exponentials.  Warp 0
-// brings in Q once and K, V through TMA rings; warp 1 issues S = Q K^T and
-// O += P V with P read from TMEM; warps 2..5 run the softmax, one row per
-// thread.  TMEM (256 columns): HD = 64 keeps P in columns of its own and takes
-// S in two 64-key halves, so the next tile's scores are computed under this
-// tile's exponentials; HD = 128 writes P over S.
+// Persistent, one CTA per SM.  An item is two neighbouring query tiles (tt tokens
+// x p heads each) of one sequence and head group: two streams that share every K
+// and V tile, each with its own softmax warpgroup.  While one stream's
+// exponentials run, the tensor core works on the other's products:
+//   PV_0(j), S_0(j+1) | PV_1(j), S_1(j+1) | ...
+// Warp 0 brings in Q, K and V by TMA, warp 1 issues the MMAs, warp 2 looks over V
+// tiles that the mask cuts, warps 4..7 and 8..11 are the softmax of streams 0 and
+// 1, one row per thread with its 128 scores in registers.  TMEM: HD = 128 writes P
+// over S (S_0 S_1 O_0 O_1); HD = 64 has columns for P, so the next scores are
+// computed as soon as these are in registers.
 //
 // Rows of other sequences never reach a result: the last key tile's V rows past
 // the sequence's end are cleared in shared memory (their P is zero, but zero
 // times an inf or NaN is not), and so are the inf or NaN elements of V in the
 // tile's masked triangle, which are added back to the rows that do see them.
+#include <type_traits>
+
 #include "attn_packed.h"
 #include "attn_packed.cuh"
 
@@ -37,82 +42,17 @@ struct PackedFwdMaps {
 
 template <int HD>
 struct PackedFwdCfg {
-  static constexpr int KS = HD <= 64 ? 2 : 1, VS = KS;  // K and V ring depth
-  static constexpr uint32_t TB = 128 * HD * 2;
   static constexpr bool SEP_P = HD <= 64;
-  static constexpr uint32_t S_COL = 0, P_COL = SEP_P ? 128 : 0, O_COL = SEP_P ? 192 : 128;
-  static constexpr uint32_t TMEM_COLS = 256;
-  static constexpr uint32_t OFF_BAR = TB * (1 + KS + VS);
-  static constexpr size_t SMEM = 1024 + OFF_BAR + 256;
+  static constexpr int QB = HD <= 64 ? 2 : 1;  // Q buffers (of two tiles)
+  static constexpr int KS = 2, VS = 2;
+  static constexpr uint32_t TB = 128 * HD * 2;
+  static constexpr uint32_t S_COL = 0, P_COL = SEP_P ? 256 : 0, P_STEP = SEP_P ? 64 : 128;
+  static constexpr uint32_t O_COL = SEP_P ? 384 : 256;
+  static constexpr uint32_t TMEM_COLS = 512;
+  static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
+  static constexpr size_t SMEM = 1024 + OFF_BAR + 512;
+  static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 };
-
-// Row maximum (NaN if any score is) of 128 raw scores in TMEM; MASK drops columns > cmax.
-template <bool MASK>
-__device__ __forceinline__ float packed_row_max(uint32_t sb, int cmax) {
-  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  auto chunk = [&](const uint32_t(&v)[16], int c) {
-    float x[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = (MASK && 16 * c + e > cmax) ? -INFINITY : __uint_as_float(v[e]);
-#pragma unroll
-    for (int e = 0; e < 16; e += 8)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = max3f_nan(m[i], x[e + 2 * i], x[e + 2 * i + 1]);
-  };
-  uint32_t a[16], b[16];
-  tmem_ld16(sb, a);
-  tmem_wait_ld_tied(a);
-#pragma unroll
-  for (int c = 0; c < 8; c += 2) {
-    tmem_ld16(sb + 16 * (c + 1), b);
-    chunk(a, c);
-    tmem_wait_ld_tied(b);
-    if (c + 2 < 8) tmem_ld16(sb + 16 * (c + 2), a);
-    chunk(b, c + 1);
-    if (c + 2 < 8) tmem_wait_ld_tied(a);
-  }
-  return max3f_nan(max3f_nan(m[0], m[1], m[2]), m[3], m[3]);
-}
-
-// P = exp2(s * sl2 - m) of the 64 columns [col0, col0 + 64): packed pairs
-// through out(c, pk) per 16-column chunk c; returns their sum.
-template <class T, bool MASK, class Out>
-__device__ __forceinline__ float packed_exp64(uint32_t sb, int col0, int cmax, float sl2, float neg_m, Out&& out) {
-  float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-  const float2 scale2 = make_float2(sl2, sl2), bias2 = make_float2(neg_m, neg_m);
-  auto chunk = [&](const uint32_t(&v)[16], int c) {
-    uint32_t pk[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 t = ffma2(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, bias2);
-      float2 pp = exp2_pair(t, (kPolyPairsFwd >> e) & 1);
-      if (MASK) {
-        const int c0 = col0 + 16 * c + 2 * e;
-        pp.x = c0 > cmax ? 0.f : pp.x;
-        pp.y = c0 + 1 > cmax ? 0.f : pp.y;
-      }
-      if (e & 1)
-        acc1 = fadd2(acc1, pp);
-      else
-        acc0 = fadd2(acc0, pp);
-      pk[e] = T::pack(pp.x, pp.y);
-    }
-    out(c, pk);
-  };
-  uint32_t a[16], b[16];
-  tmem_ld16(sb + col0, a);
-  tmem_wait_ld_tied(a);
-#pragma unroll
-  for (int c = 0; c < 4; c += 2) {
-    tmem_ld16(sb + col0 + 16 * (c + 1), b);
-    chunk(a, c);
-    tmem_wait_ld_tied(b);
-    if (c + 2 < 4) tmem_ld16(sb + col0 + 16 * (c + 2), a);
-    chunk(b, c + 1);
-    if (c + 2 < 4) tmem_wait_ld_tied(a);
-  }
-  return (acc0.x + acc0.y) + (acc1.x + acc1.y);
-}
 
 // Clears the inf and NaN elements of rows [r0, r1) of a V tile (one warp); true if there were any.
 template <int HD, class T>
@@ -143,79 +83,81 @@ __device__ __forceinline__ bool clear_nonfinite(uint32_t tile, int r0, int r1, i
   return true;
 }
 
+// One item: the query tiles [t0, t0 + tt) and, with two streams, [t0 + tt, t0 + 2 tt) of a sequence.
+struct FwdItem {
+  int seq0, len, t0, end, h0, kvh;
+  int nkv[2];  // key tiles of each stream (0: no such tile)
+  int n;       // the larger: stream 1 never has fewer, unless it is not there
+  __device__ FwdItem() {}
+  __device__ FwdItem(const PackedFwdParams& p, int idx) {
+    const int rows = p.d.rows[LIST_FWD];
+    const PackedTile<true> it(p.plan.list[LIST_FWD], idx, p.d.hg, rows);
+    seq0 = it.seq0;
+    len = it.len;
+    t0 = it.tile * rows;
+    end = min(t0 + rows, len);
+    h0 = it.head * p.d.p;
+    kvh = h0 / (p.d.Hq / p.d.Hkv);
+    nkv[0] = (min(t0 + p.d.tt, len) + 127) >> 7;
+    nkv[1] = end > t0 + p.d.tt ? (end + 127) >> 7 : 0;
+    n = max(nkv[0], nkv[1]);
+  }
+};
+
 template <int HD, class T>
-__global__ void __launch_bounds__(192, 2) packed_fwd_kernel(const __grid_constant__ PackedFwdMaps maps,
+__global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constant__ PackedFwdMaps maps,
                                                             const __grid_constant__ PackedFwdParams p) {
   using Cfg = PackedFwdCfg<HD>;
   using Tile = HeadTile<HD>;
-  constexpr int KS = Cfg::KS, VS = Cfg::VS;
+  constexpr int KS = Cfg::KS, VS = Cfg::VS, QB = Cfg::QB;
   constexpr uint32_t TB = Cfg::TB;
   constexpr uint32_t IDESC_S = idesc_16bit(T::FMT, 128, 128, 0, 0);
-  constexpr uint32_t IDESC_SH = idesc_16bit(T::FMT, 128, 64, 0, 0);  // (SEP_P) one 64-key half of S
   constexpr uint32_t IDESC_O = idesc_16bit(T::FMT, 128, HD, 0, 1);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t sQ = smem_u32(smem);
-  const uint32_t sK = sQ + TB;       // KS K tiles
-  const uint32_t sV = sK + KS * TB;  // VS V tiles
+  const uint32_t base = smem_u32(smem);
+  auto sQ = [&](int b, int x) { return base + (2 * b + x) * TB; };
+  auto sK = [&](int s) { return base + Cfg::OFF_K + s * TB; };
+  auto sV = [&](int s) { return base + Cfg::OFF_V + s * TB; };
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   const uint32_t b0 = smem_u32(bars);
-  const uint32_t q_full = b0;
-  auto k_full = [&](int s) { return b0 + 8u * (1 + s); };
-  auto k_empty = [&](int s) { return b0 + 8u * (1 + KS + s); };
-  auto v_full = [&](int s) { return b0 + 8u * (1 + 2 * KS + s); };
-  auto v_empty = [&](int s) { return b0 + 8u * (1 + 2 * KS + VS + s); };
-  const uint32_t s_full = b0 + 8u * (1 + 2 * KS + 2 * VS);  // S_j (SEP_P: its keys [0, 64)) computed
-  const uint32_t p_full = s_full + 8;                        // P_j written
-  const uint32_t o_bar = s_full + 16;                        // every MMA done
-  const uint32_t drain_bar = s_full + 24;
-  const uint32_t s_empty = s_full + 32;    // (SEP_P) the softmax has read the half [0, 64)
-  const uint32_t pv_done = s_full + 40;    // (SEP_P) PV_j done
-  const uint32_t s_full_b = s_full + 48;   // (SEP_P) the half [64, 128)
-  const uint32_t s_empty_b = s_full + 56;
-  const uint32_t v_raw = s_full + 64;      // a V tile that warp 0 looks over before the MMA may read it
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 1 + 2 * KS + 2 * VS + 9);
-  uint32_t* bad_slot = tmem_slot + 1;
+  auto q_full = [&](int b) { return b0 + 8u * b; };
+  auto q_empty = [&](int b) { return b0 + 8u * (2 + b); };
+  auto k_full = [&](int s) { return b0 + 8u * (4 + s); };
+  auto k_empty = [&](int s) { return b0 + 8u * (6 + s); };
+  auto v_full = [&](int s) { return b0 + 8u * (8 + s); };
+  auto v_empty = [&](int s) { return b0 + 8u * (10 + s); };
+  auto v_raw = [&](int s) { return b0 + 8u * (12 + s); };    // landed, for warp 2 to look over
+  auto s_full = [&](int x) { return b0 + 8u * (14 + x); };   // S_x(j) computed
+  auto s_empty = [&](int x) { return b0 + 8u * (16 + x); };  // (SEP_P) and in registers
+  auto p_full = [&](int x) { return b0 + 8u * (18 + x); };   // P_x(j) written
+  auto pv_done = [&](int x) { return b0 + 8u * (20 + x); };  // (SEP_P) PV_x(j) done
+  auto o_full = [&](int x) { return b0 + 8u * (22 + x); };   // an item's O_x complete
+  auto o_empty = [&](int x) { return b0 + 8u * (24 + x); };  // and read out
+  const uint32_t drain_bar = b0 + 8u * 26;
+  const Feed feed{b0 + 8u * 28, b0 + 8u * 32, reinterpret_cast<int*>(bars + 36)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
+  volatile int* bad = reinterpret_cast<int*>(bars + 40);  // per item (mod 4) and stream: V held inf or NaN behind the mask
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int s = 0; s < KS; ++s) {
-      mbar_init(k_full(s), 1);
-      mbar_init(k_empty(s), 1);
+    for (int i = 0; i < 16; ++i) mbar_init(b0 + 8u * i, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_empty(x), 128);
+      mbar_init(p_full(x), 128);
+      mbar_init(pv_done(x), 1);
+      mbar_init(o_full(x), 1);
+      mbar_init(o_empty(x), 128);
     }
-    for (int s = 0; s < VS; ++s) {
-      mbar_init(v_full(s), 1);
-      mbar_init(v_empty(s), 1);
-    }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 128);
-    mbar_init(o_bar, 1);
     mbar_init(drain_bar, 1);
-    mbar_init(s_empty, 128);
-    mbar_init(pv_done, 1);
-    mbar_init(s_full_b, 1);
-    mbar_init(s_empty_b, 128);
-    mbar_init(v_raw, 1);
-    *bad_slot = 0;
+    for (int i = 0; i < Feed::SLOTS; ++i) {
+      mbar_init(feed.full + 8u * i, 1);
+      mbar_init(feed.empty + 8u * i, 10);  // MMA, warp 2, eight softmax warps
+    }
     fence_mbar_init();
   }
-  pdl_wait();
-
-  const PackedHeader hd = *p.plan.head;
-  zero_outside(static_cast<uint4*>(p.o), p.d.total, hd.first, hd.end, (long long)p.d.Hq * p.d.N / 8, blockIdx.x,
-               gridDim.x, threadIdx.x, blockDim.x);
-  if (int(blockIdx.x) / p.d.hg >= hd.n_q) return;
-  const PackedTile<true> item(p.plan.q_items, blockIdx.x, p.d.hg, p.d.tt);
-  const int h0 = item.head * p.d.p;  // first head
-  const int kvh = h0 / (p.d.Hq / p.d.Hkv);
-  const int seq0 = item.seq0, len = item.len;
-  const int t0 = item.tile * p.d.tt;
-  const int t1 = min(t0 + p.d.tt, len);
-  const int nkv = (t1 + 127) >> 7;
-
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
     tmem_relinquish();
@@ -224,289 +166,374 @@ __global__ void __launch_bounds__(192, 2) packed_fwd_kernel(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
   Guard g(p.status, KID_PACKED_FWD);
+  auto finish = [&]() {
+    tc_fence_before();
+    named_bar_sync(1, 384);
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, Cfg::TMEM_COLS);
+    }
+  };
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
-    const bool lead = lane == 0;
-    if (lead) {
-      tma_prefetch_desc(&maps.q);
-      tma_prefetch_desc(&maps.k);
-      tma_prefetch_desc(&maps.v);
-      mbar_expect_tx(q_full, uint32_t(p.d.p * p.d.tt) * 128 * Tile::NCHUNK);
+  if (warp < 4) {
+    reg_dealloc<Cfg::REG_REST>();
+    if (warp == 0) {
+      // ---------------- TMA producer ----------------
+      if (lane == 0) {
+        const int n_items = p.plan.head->n[LIST_FWD] * p.d.hg;
+        const uint32_t box = uint32_t(p.d.p * p.d.tt) * 128 * Tile::NCHUNK;
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+        int qpar[2] = {-1, -1}, kpar[KS], vpar[VS];
+        for (int s = 0; s < KS; ++s) kpar[s] = -1;
+        for (int s = 0; s < VS; ++s) vpar[s] = -1;
+        int n = 0, idx = blockIdx.x;
+        for (int item = 0; g.ok; ++item) {
+          feed.put(item, idx < n_items ? idx : -1, g);
+          if (idx >= n_items) break;
+          const int after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_FWD], 1);
+          const FwdItem w(p, idx);
+          const int qb = item % QB;
+          if (item >= QB && !mbar_wait(q_empty(qb), uint32_t((item / QB - 1) & 1), g, 1)) break;
+          mbar_expect_tx(q_full(qb), w.nkv[1] ? 2 * box : box);
+          for (int x = 0; x < (w.nkv[1] ? 2 : 1); ++x)
 #pragma unroll
-      for (int c = 0; c < Tile::NCHUNK; ++c) tma_load_3d(sQ + c * 16384, &maps.q, q_full, c * 64, h0, seq0 + t0);
-    }
-    int kpar[KS], vpar[VS];
-    for (int s = 0; s < KS; ++s) kpar[s] = -1;
-    for (int s = 0; s < VS; ++s) vpar[s] = -1;
-    int raw = 0;  // uses of v_raw
-    for (int j = 0; j < nkv && g.ok; ++j) {
-      const int sk = j % KS, sv = j % VS;
-      const uint32_t pk = (j / KS) & 1, pv = (j / VS) & 1;
-      // Rows [from, to) of this V tile are masked for some rows of the query
-      // tile only, rows [to, 128) for all of them.
-      const int from = max(t0 + 1 - 128 * j, 0), to = min(t1 - 128 * j, 128);
-      const bool look = from < 128;
-      if (lead) {
-        if (mbar_wait(k_empty(sk), pk ^ 1, g, 1)) {
-          mbar_expect_tx(k_full(sk), TB);
+            for (int c = 0; c < Tile::NCHUNK; ++c)
+              tma_load_3d(sQ(qb, x) + c * 16384, &maps.q, q_full(qb), c * 64, w.h0, w.seq0 + w.t0 + x * p.d.tt);
+          qpar[qb] = (item / QB) & 1;
+          for (int j = 0; j < w.n; ++j, ++n) {
+            const int sk = n % KS, sv = n % VS;
+            const uint32_t pk = (n / KS) & 1, pv = (n / VS) & 1;
+            if (!mbar_wait(k_empty(sk), pk ^ 1, g, 2)) break;
+            mbar_expect_tx(k_full(sk), TB);
 #pragma unroll
-          for (int c = 0; c < Tile::NCHUNK; ++c)
-            tma_load_3d(sK + sk * TB + c * 16384, &maps.k, k_full(sk), c * 64, kvh, seq0 + j * 128);
-          kpar[sk] = int(pk);
-        }
-        if (mbar_wait(v_empty(sv), pv ^ 1, g, 9)) {
-          const uint32_t full = look ? v_raw : v_full(sv);
-          mbar_expect_tx(full, TB);
+            for (int c = 0; c < Tile::NCHUNK; ++c)
+              tma_load_3d(sK(sk) + c * 16384, &maps.k, k_full(sk), c * 64, w.kvh, w.seq0 + j * 128);
+            kpar[sk] = int(pk);
+            if (!mbar_wait(v_empty(sv), pv ^ 1, g, 3)) break;
+            mbar_expect_tx(v_raw(sv), TB);
 #pragma unroll
-          for (int c = 0; c < Tile::NCHUNK; ++c)
-            tma_load_3d(sV + sv * TB + c * 16384, &maps.v, full, c * 64, kvh, seq0 + j * 128);
-          vpar[sv] = int(pv);
-        }
-      }
-      g.ok = __all_sync(0xffffffffu, g.ok);
-      if (look && g.ok) {
-        g.ok = __all_sync(0xffffffffu, mbar_wait(v_raw, raw & 1, g, 13));
-        ++raw;
-        if (!g.ok) break;
-        zero_rows<HD>(sV + sv * TB, to, lane);
-        if (clear_nonfinite<HD, T>(sV + sv * TB, from, to, lane) && lead) *bad_slot = 1;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lead) mbar_arrive(v_full(sv));
-      }
-    }
-    if (lead) {
-      if (!g.ok) {
-        mbar_drain(q_full, 0);
-        for (int s = 0; s < KS; ++s)
-          if (kpar[s] >= 0) mbar_drain(k_full(s), uint32_t(kpar[s]));
-        for (int s = 0; s < VS; ++s)
-          if (vpar[s] >= 0) mbar_drain(v_full(s), uint32_t(vpar[s]));
-        mbar_drain(v_raw, uint32_t(raw & 1));
-      } else {
-        // The MMA warp's last releases have landed before this CTA's shared memory goes away.
-        for (int s = 0; s < KS; ++s)
-          if (kpar[s] >= 0) mbar_wait(k_empty(s), uint32_t(kpar[s]), g, 14);
-        for (int s = 0; s < VS; ++s)
-          if (vpar[s] >= 0) mbar_wait(v_empty(s), uint32_t(vpar[s]), g, 15);
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (elect_one()) {
-      bool any = false;
-      auto issue_pv = [&](int j) {
-        const int sv = j % VS;
-#pragma unroll
-        for (int kc = 0; kc < 8; ++kc)
-          mma_ts(tmem + Cfg::O_COL, tmem + Cfg::P_COL + kc * 8, Tile::mnmajor(sV + sv * TB, 128, kc), IDESC_O,
-                 (j > 0 || kc > 0) ? 1u : 0u);
-        mma_commit(v_empty(sv));
-      };
-      if constexpr (Cfg::SEP_P) {
-        auto issue_half = [&](int j, int hf) {
-          const int sk = j % KS;
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            mma_ss(tmem + Cfg::S_COL + 64 * hf, Tile::kmajor(sQ, 128, kk),
-                   Tile::kmajor(sK + sk * TB + hf * 64 * Tile::SWB, 128, kk), IDESC_SH, kk > 0 ? 1u : 0u);
-          if (hf) mma_commit(k_empty(sk));
-          mma_commit(hf ? s_full_b : s_full);
-        };
-        if (mbar_wait(q_full, 0, g, 5) && mbar_wait(k_full(0), 0, g, 2)) {
-          tc_fence_after();
-          issue_half(0, 0);
-          issue_half(0, 1);
-          any = true;
-          for (int j = 0; j < nkv; ++j) {
-            if (j + 1 < nkv) {  // each half of S_{j+1} as soon as that half of S_j has been read
-              if (!mbar_wait(s_empty, j & 1, g, 10)) break;
-              if (!mbar_wait(k_full((j + 1) % KS), ((j + 1) / KS) & 1, g, 2)) break;
-              tc_fence_after();
-              issue_half(j + 1, 0);
-              if (!mbar_wait(s_empty_b, j & 1, g, 16)) break;
-              tc_fence_after();
-              issue_half(j + 1, 1);
-            }
-            if (!mbar_wait(p_full, j & 1, g, 3)) break;
-            if (!mbar_wait(v_full(j % VS), (j / VS) & 1, g, 4)) break;
-            tc_fence_after();
-            issue_pv(j);
-            mma_commit(pv_done);
+            for (int c = 0; c < Tile::NCHUNK; ++c)
+              tma_load_3d(sV(sv) + c * 16384, &maps.v, v_raw(sv), c * 64, w.kvh, w.seq0 + j * 128);
+            vpar[sv] = int(pv);
           }
-          if (g.ok) mma_commit(o_bar);
+          idx = after;
         }
-      } else if (mbar_wait(q_full, 0, g, 5)) {
-        for (int j = 0; j < nkv; ++j) {
-          const int sk = j % KS;
-          if (!mbar_wait(k_full(sk), (j / KS) & 1, g, 2)) break;
+        if (!g.ok) {
+          for (int b = 0; b < QB; ++b)
+            if (qpar[b] >= 0) mbar_drain(q_full(b), uint32_t(qpar[b]));
+          for (int s = 0; s < KS; ++s)
+            if (kpar[s] >= 0) mbar_drain(k_full(s), uint32_t(kpar[s]));
+          for (int s = 0; s < VS; ++s)
+            if (vpar[s] >= 0) mbar_drain(v_raw(s), uint32_t(vpar[s]));
+        } else {
+          // The MMA warp's last releases have landed before this CTA's shared memory goes away.
+          for (int b = 0; b < QB; ++b)
+            if (qpar[b] >= 0) mbar_wait(q_empty(b), uint32_t(qpar[b]), g, 4);
+          for (int s = 0; s < KS; ++s)
+            if (kpar[s] >= 0) mbar_wait(k_empty(s), uint32_t(kpar[s]), g, 5);
+          for (int s = 0; s < VS; ++s)
+            if (vpar[s] >= 0) mbar_wait(v_empty(s), uint32_t(vpar[s]), g, 6);
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      if (elect_one()) {
+        bool any = false;
+        int done[2] = {0, 0};  // steps of each stream so far (parities of p_full, s_empty)
+        auto get = [&](int item, FwdItem& w) -> bool {
+          const int idx = feed.get(item, g);
+          if (idx < 0) return false;
+          w = FwdItem(p, idx);
+          return true;
+        };
+        // S_x(j) of an item whose first K tile is number k0; the last stream to use the tile gives it back.
+        auto issue_s = [&](const FwdItem& w, int item, int k0, int x, int j) -> bool {
+          const int qb = item % QB, sk = (k0 + j) % KS;
+          if (j == 0 && !mbar_wait(q_full(qb), (item / QB) & 1, g, 7)) return false;
+          if (!mbar_wait(k_full(sk), ((k0 + j) / KS) & 1, g, 8)) return false;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
-            mma_ss(tmem + Cfg::S_COL, Tile::kmajor(sQ, 128, kk), Tile::kmajor(sK + sk * TB, 128, kk), IDESC_S,
+            mma_ss(tmem + Cfg::S_COL + 128 * x, Tile::kmajor(sQ(qb, x), 128, kk), Tile::kmajor(sK(sk), 128, kk), IDESC_S,
                    kk > 0 ? 1u : 0u);
-          mma_commit(k_empty(sk));
-          mma_commit(s_full);
+          mma_commit(s_full(x));
+          if (x == 1 || j >= w.nkv[1]) mma_commit(k_empty(sk));
+          if (j + 1 == w.n && (x == 1 || !w.nkv[1])) mma_commit(q_empty(qb));  // the item's last read of Q
           any = true;
-          if (!mbar_wait(p_full, j & 1, g, 3)) break;
-          if (!mbar_wait(v_full(j % VS), (j / VS) & 1, g, 4)) break;
-          tc_fence_after();
-          issue_pv(j);
-        }
-        if (g.ok) mma_commit(o_bar);
-      }
-      if (!g.ok && any) {
-        mma_commit(drain_bar);
-        mbar_drain(drain_bar, 0);
-      }
-    }
-  } else {
-    // ---------------- softmax + epilogue: warps 2..5 ----------------
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;  // row of the query tile
-    const int t = t0 + r / p.d.p;       // token within the sequence
-    const bool live = r < p.d.p * p.d.tt && t < t1;
-    const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
-    const uint32_t sb = lane_base + Cfg::S_COL;
-    const float sl2 = p.scale_log2;
-    float m_run = -INFINITY, l_run = 0.f;  // m_run in scaled log2 units
-    bool ok = true, nan_row = false;
-    // Takes S_j's row maximum mx (raw) into the running maximum.  Lazy: the
-    // reference moves only when the maximum grows by more than 8 (log2 units), so
-    // P stays <= 2^8; O and the sum are rescaled only then.  `o_ready` makes O stable.
-    auto rescale = [&](float mx_raw, int j, auto&& o_ready) {
-      const float mx = mx_raw * sl2;
-      nan_row |= mx != mx;
-      const bool need = mx > m_run + 8.0f || (m_run == -INFINITY && mx > -INFINITY);
-      if (__any_sync(0xffffffffu, need)) {
-        const float m_new = need ? mx : m_run;
-        const float alpha = need ? ex2(m_run - m_new) : 1.0f;  // 0 when m_run = -inf
-        if (j > 0) {
-          if (!o_ready()) return;
+          return true;
+        };
+        FwdItem w;
+        int k0 = 0, outs[2] = {0, 0};  // K tile number at the item's start; items that each stream has had
+        bool have = get(0, w);
+        if (have && issue_s(w, 0, 0, 0, 0) && w.nkv[1]) issue_s(w, 0, 0, 1, 0);
+        for (int item = 0; have && g.ok; ++item) {
+          for (int j = 0; j < w.n && g.ok; ++j) {
+            const int sv = (k0 + j) % VS;
 #pragma unroll
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t ov[16];
-            tmem_load16(lane_base + Cfg::O_COL + c, ov);
+            for (int x = 0; x < 2; ++x) {
+              if (j >= w.nkv[x]) continue;
+              const bool more = j + 1 < w.nkv[x];
+              if (Cfg::SEP_P && more) {  // the next scores as soon as these are in registers
+                if (!mbar_wait(s_empty(x), done[x] & 1, g, 9) || !issue_s(w, item, k0, x, j + 1)) break;
+              }
+              if (!mbar_wait(p_full(x), done[x] & 1, g, 10)) break;
+              if (!mbar_wait(v_full(sv), ((k0 + j) / VS) & 1, g, 11)) break;
+              if (j == 0 && outs[x] > 0 && !mbar_wait(o_empty(x), (outs[x] - 1) & 1, g, 12)) break;
+              tc_fence_after();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-            tmem_st16(lane_base + Cfg::O_COL + c, ov);
+              for (int kc = 0; kc < 8; ++kc)
+                mma_ts(tmem + Cfg::O_COL + HD * x, tmem + Cfg::P_COL + Cfg::P_STEP * x + kc * 8, Tile::mnmajor(sV(sv), 128, kc),
+                       IDESC_O, (j > 0 || kc > 0) ? 1u : 0u);
+              if (Cfg::SEP_P) mma_commit(pv_done(x));
+              if (x == 1 || j >= w.nkv[1]) mma_commit(v_empty(sv));
+              if (!more) {
+                mma_commit(o_full(x));
+                ++outs[x];
+              }
+              ++done[x];
+              if (!Cfg::SEP_P && more && !issue_s(w, item, k0, x, j + 1)) break;
+            }
+          }
+          if (!g.ok) break;
+          k0 += w.n;
+          FwdItem nx;
+          have = get(item + 1, nx);
+          if (have) {
+            // SEP_P: the last scores must be in registers before the next item's are written.
+            for (int x = 0; x < (nx.nkv[1] ? 2 : 1); ++x) {
+              if (Cfg::SEP_P && done[x] > 0 && !mbar_wait(s_empty(x), (done[x] - 1) & 1, g, 13)) break;
+              if (!issue_s(nx, item + 1, k0, x, 0)) break;
+            }
+            w = nx;
           }
         }
-        l_run *= alpha;
-        m_run = m_new;
+        if (!g.ok && any) {
+          mma_commit(drain_bar);
+          mbar_drain(drain_bar, 0);
+        }
       }
-    };
-    for (int j = 0; j < nkv && ok; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, g, 6));
-      if (!ok) break;
-      const bool mask = 128 * j + 127 > t0;
-      const int cmax = t - 128 * j;  // last column this row sees
-      if constexpr (Cfg::SEP_P) {
-        ok = __all_sync(0xffffffffu, mbar_wait(s_full_b, j & 1, g, 17));
+    } else if (warp == 2) {
+      // ---------------- V tiles: passed on, or looked over where the mask cuts them ----------------
+      int n = 0;
+      for (int item = 0; g.ok; ++item) {
+        const int idx = feed.get_warp(item, g, lane);
+        if (!g.ok || idx < 0) break;
+        const FwdItem w(p, idx);
+        bool found = false;
+        for (int j = 0; j < w.n; ++j, ++n) {
+          const int sv = n % VS;
+          g.ok = __all_sync(0xffffffffu, mbar_wait(v_raw(sv), (n / VS) & 1, g, 14));
+          if (!g.ok) break;
+          // Rows [from, to) of the tile are masked for some rows of the item only, rows [to, 128) for all of them.
+          const int from = max(w.t0 + 1 - 128 * j, 0), to = min(w.end - 128 * j, 128);
+          if (from < 128) {
+            zero_rows<HD>(sV(sv), to, lane);
+            found |= clear_nonfinite<HD, T>(sV(sv), from, to, lane);
+            fence_proxy_async_smem();
+          }
+          if (lane == 0)  // with the stream's last V tile, which its O waits for
+            for (int x = 0; x < 2; ++x)
+              if (j + 1 == w.nkv[x]) bad[(item & 3) * 2 + x] = found;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_full(sv));
+        }
+      }
+    }
+    finish();
+    return;
+  }
+  reg_alloc<Cfg::REG_SOFTMAX>();
+  // ---------------- softmax + epilogue: stream x, row r ----------------
+  {
+    const PackedHeader hd = *p.plan.head;
+    zero_outside(static_cast<uint4*>(p.o), p.d.total, hd.first, hd.end, (long long)p.d.Hq * p.d.N / 8, blockIdx.x,
+                 gridDim.x, threadIdx.x - 128, 256);
+    const int x = (warp - 4) >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const int tok = r / p.d.p, hr = r - tok * p.d.p;
+    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t st = lane_base + Cfg::S_COL + 128 * x, pt = lane_base + Cfg::P_COL + Cfg::P_STEP * x;
+    const uint32_t ot = lane_base + Cfg::O_COL + HD * x;
+    const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+    bool ok = true;
+    int n = 0, outs = 0;  // steps and items of this stream
+    for (int item = 0; ok; ++item) {
+      const int idx = feed.get_warp(item, g, lane);
+      ok = g.ok;
+      if (!ok || idx < 0) break;
+      const FwdItem w(p, idx);
+      const int nkv = x ? w.nkv[1] : w.nkv[0];
+      if (!nkv) continue;
+      const int first = w.t0 + x * p.d.tt;  // the tile's first token
+      const int t = first + tok;
+      const bool live = tok < p.d.tt && t < w.end;
+      float m_run = -INFINITY, l_run = 0.f;  // m_run in scaled log2 units
+      bool nan_row = false;
+#pragma unroll 1
+      for (int j = 0; j < nkv; ++j, ++n) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full(x), n & 1, g, 15));
         if (!ok) break;
         tc_fence_after();
-        bool pv_seen = (j == 0);  // PV_{j-1} has completed: O and the P columns are free
-        auto wait_pv = [&]() -> bool {
-          ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (j - 1) & 1, g, 11));
-          if (ok) tc_fence_after();
-          pv_seen = true;
-          return ok;
-        };
-        rescale(mask ? packed_row_max<true>(sb, cmax) : packed_row_max<false>(sb, cmax), j, wait_pv);
-        if (!ok) break;
-        const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
-        // Keys [0, 64), then [64, 128): one loop, so the exponential code exists once per mask.
-#pragma unroll 1
-        for (int hh = 0; hh < 2; ++hh) {
-          uint32_t pk[32];
-          auto keep = [&](int c, const uint32_t(&w)[8]) {
+        float s[128];
+        {
+          uint32_t a[32], b[32], c[32], d[32];
+          tmem_ld32(st, a);
+          tmem_ld32(st + 32, b);
+          tmem_ld32(st + 64, c);
+          tmem_ld32(st + 96, d);
+          tmem_wait_ld_tied2x32(a, b);
+          reg_tie(c);
+          reg_tie(d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pk[8 * c + e] = w[e];
-          };
-          l_run += mask ? packed_exp64<T, true>(sb, 64 * hh, cmax, sl2, neg_m, keep)
-                        : packed_exp64<T, false>(sb, 64 * hh, cmax, sl2, neg_m, keep);
+          for (int e = 0; e < 32; ++e) {
+            s[e] = __uint_as_float(a[e]);
+            s[32 + e] = __uint_as_float(b[e]);
+            s[64 + e] = __uint_as_float(c[e]);
+            s[96 + e] = __uint_as_float(d[e]);
+          }
+        }
+        if (Cfg::SEP_P) {
           tc_fence_before();
-          mbar_arrive(hh ? s_empty_b : s_empty);
-          if (!pv_seen && !wait_pv()) break;
+          mbar_arrive(s_empty(x));
+        }
+        const bool mask = 128 * j + 127 > first;
+        if (mask) {
+          const int cmax = t - 128 * j;  // last column this row sees
 #pragma unroll
-          for (int q2 = 0; q2 < 2; ++q2)
-            tmem_st16(lane_base + Cfg::P_COL + 32 * hh + 16 * q2, *reinterpret_cast<const uint32_t(*)[16]>(pk + 16 * q2));
-          tmem_st_wait();  // the next half rewrites the registers of pk
+          for (int e = 0; e < 128; ++e) s[e] = e > cmax ? -INFINITY : s[e];
         }
-        if (!ok) break;
-      } else {
-        tc_fence_after();
-        // S_j was issued after PV_{j-1} on the in-order tensor pipe: O is stable.
-        rescale(mask ? packed_row_max<true>(sb, cmax) : packed_row_max<false>(sb, cmax), j, [] { return true; });
-        const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+        float m[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int e = 4; e < 124; e += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m[i] = max3f_nan(m[i], s[e + 2 * i], s[e + 2 * i + 1]);
+        m[0] = max3f_nan(m[0], s[124], s[125]);
+        m[1] = max3f_nan(m[1], s[126], s[127]);
+        const float mx = max3f_nan(max3f_nan(m[0], m[1], m[2]), m[3], m[3]) * p.scale_log2;
+        nan_row |= mx != mx;
+        // PV(j - 1) is done: O is stable and the P columns are free.  (HD = 128: S(j)
+        // was issued after it on the in-order tensor pipe.)
+        if (Cfg::SEP_P && n > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(pv_done(x), (n - 1) & 1, g, 16));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        // Lazy: the reference moves only when the maximum grows by more than 8 (log2
+        // units), so P stays <= 2^8; O and the sum are rescaled only then.
+        const bool need = mx > m_run + 8.0f || (m_run == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, need)) {
+          const float m_new = need ? mx : m_run;
+          const float alpha = need ? ex2(m_run - m_new) : 1.0f;  // 0 when m_run = -inf
+          if (j > 0) {
 #pragma unroll 1
-        for (int hh = 0; hh < 2; ++hh) {
-          auto store = [&](int c, const uint32_t(&w)[8]) { tmem_st8(sb + 32 * hh + 8 * c, w); };
-          l_run += mask ? packed_exp64<T, true>(sb, 64 * hh, cmax, sl2, neg_m, store)
-                        : packed_exp64<T, false>(sb, 64 * hh, cmax, sl2, neg_m, store);
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t ov[16];
+              tmem_load16(ot + c, ov);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tmem_st16(ot + c, ov);
+            }
+          }
+          l_run *= alpha;
+          m_run = m_new;
         }
+        const float nm = m_run == -INFINITY ? 0.f : -m_run;
+        const float2 neg_m = make_float2(nm, nm);
+        float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
+        // In a masked tile every exponential runs on MUFU, which turns -inf into exactly 0.
+        auto exps = [&](auto masked) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 pp = exp2_pair(ffma2(make_float2(s[16 * c + 2 * e], s[16 * c + 2 * e + 1]), sl2, neg_m),
+                                          !masked() && ((kPolyPairsFwd >> e) & 1));
+              if (e & 1)
+                acc1 = fadd2(acc1, pp);
+              else
+                acc0 = fadd2(acc0, pp);
+              pk[e] = T::pack(pp.x, pp.y);
+            }
+            tmem_st8(pt + 8 * c, pk);
+          }
+        };
+        if (mask)
+          exps(std::true_type());
+        else
+          exps(std::false_type());
+        l_run += (acc0.x + acc0.y) + (acc1.x + acc1.y);
         tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_full(x));
+      }
+      if (!ok) break;
+      // ---- epilogue: O / l ----
+      ok = __all_sync(0xffffffffu, mbar_wait(o_full(x), outs & 1, g, 17));
+      if (!ok) break;
+      tc_fence_after();
+      ++outs;
+      float f[HD];
+#pragma unroll
+      for (int c = 0; c < HD; c += 64) {
+        uint32_t a[32], b[32];
+        tmem_ld32(ot + c, a);
+        tmem_ld32(ot + c + 32, b);
+        tmem_wait_ld_tied2x32(a, b);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          f[c + e] = __uint_as_float(a[e]);
+          f[c + 32 + e] = __uint_as_float(b[e]);
+        }
       }
       tc_fence_before();
-      mbar_arrive(p_full);
-    }
-    // ---- epilogue: O / l ----
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_bar, 0, g, 8));
-    if (ok && Cfg::SEP_P) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (nkv - 1) & 1, g, 12));
-    if (ok) {
-      tc_fence_after();
-      const bool bad = *reinterpret_cast<volatile uint32_t*>(bad_slot) != 0;
+      mbar_arrive(o_empty(x));
       nan_row |= m_run == -INFINITY;  // no finite score: 0 / 0
       const float inv_l = nan_row ? __int_as_float(0x7fffffff) : 1.0f / l_run;
-      const int h = h0 + r % p.d.p;
-      const long long row = (long long)(seq0 + t) * p.d.Hq + h;
-      uint16_t* orow = static_cast<uint16_t*>(p.o) + row * p.d.N;
-#pragma unroll 1
-      for (int c = 0; c < HD; c += 16) {
-        uint32_t ov[16];
-        __syncwarp();
-        tmem_load16(lane_base + Cfg::O_COL + c, ov);
-        float f[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(ov[e]) * inv_l;
-        if (bad && live) {  // the inf and NaN elements that were cleared, for the rows that see them
-          for (int key = t0 + 1; key <= t; ++key) {
-            const uint16_t* vr = static_cast<const uint16_t*>(p.v) + (long long)(seq0 + key) * p.v_tok + kvh * p.v_head;
-            for (int e = 0; e < 16; ++e)
-              if (c + e < p.d.N && half_nonfinite<T>(vr[c + e])) f[e] += T::lo(vr[c + e]);
-          }
-        }
-        if (live) {
-          if (c < p.d.N)
-            st_global_v4(orow + c, T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7]));
-          if (c + 8 < p.d.N)
-            st_global_v4(orow + c + 8, T::pack(f[8], f[9]), T::pack(f[10], f[11]), T::pack(f[12], f[13]),
-                         T::pack(f[14], f[15]));
+      for (int e = 0; e < HD; ++e) f[e] *= inv_l;
+      if (bad[(item & 3) * 2 + x] && live) {  // the inf and NaN elements that were cleared, for the rows that see them
+#pragma unroll 1
+        for (int key = w.t0 + 1; key <= t; ++key) {
+          const uint16_t* vr = static_cast<const uint16_t*>(p.v) + (long long)(w.seq0 + key) * p.v_tok + w.kvh * p.v_head;
+#pragma unroll
+          for (int e = 0; e < HD; ++e)
+            if (e < p.d.N && half_nonfinite<T>(vr[e])) f[e] += T::lo(vr[e]);
         }
       }
-      if (live) p.lse2[row] = nan_row ? __int_as_float(0x7fffffff) : m_run + __log2f(l_run);
+      const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
+      if (live) {
+        uint16_t* orow = static_cast<uint16_t*>(p.o) + row * p.d.N;
+#pragma unroll
+        for (int c = 0; c < HD; c += 8)
+          if (c < p.d.N)
+            st_global_v4(orow + c, T::pack(f[c], f[c + 1]), T::pack(f[c + 2], f[c + 3]), T::pack(f[c + 4], f[c + 5]),
+                         T::pack(f[c + 6], f[c + 7]));
+        p.lse2[row] = nan_row ? __int_as_float(0x7fffffff) : m_run + __log2f(l_run);
+      }
+      __syncwarp();
     }
+    // The last pv_done has landed before this CTA's shared memory goes away.
+    if (Cfg::SEP_P && ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done(x), (n - 1) & 1, g, 18));
     if (!ok) g.ok = false;
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, Cfg::TMEM_COLS);
+    finish();
   }
 }
 
 template <int HD, class T>
 static int launch_packed_fwd(const PackedFwdMaps& maps, const PackedFwdParams& p, cudaStream_t st) {
   using Cfg = PackedFwdCfg<HD>;
+  static_assert(Cfg::SMEM <= 232448, "shared memory");
   auto kern = packed_fwd_kernel<HD, T>;
   if (!smem_attr_set(reinterpret_cast<const void*>(kern), int(Cfg::SMEM)))
     return set_error(MEA_ERR_CUDA, "cudaFuncSetAttribute(packed_fwd) failed");
   cudaLaunchAttribute attr;
-  const cudaLaunchConfig_t cfg = packed_launch(p.d.cap_q * p.d.hg, 192, Cfg::SMEM, st, &attr);
+  const long long items = (long long)p.d.cap[LIST_FWD] * p.d.hg;
+  const cudaLaunchConfig_t cfg = packed_launch(int(items < num_sms() ? items : num_sms()), 384, Cfg::SMEM, st, &attr);
   cudaLaunchKernelEx(&cfg, kern, maps, p);
   return check_launch("packed_fwd_kernel");
 }
@@ -549,7 +576,7 @@ extern "C" int mea_packed_attention_forward(const mea_packed_dims* d, const void
   p.o = o;
   p.lse2 = lse2;
   p.status = status;
-  if (pd.cap_q == 0) {
+  if (pd.cap[LIST_FWD] == 0) {
     // n_seqs = 0: no query tile can exist, every row of o is outside.
     if (cudaMemsetAsync(o, 0, size_t(pd.total) * pd.Hq * pd.N * 2, st) != cudaSuccess)
       return set_error(MEA_ERR_CUDA, "packed attention: clearing o failed");

@@ -65,14 +65,13 @@ __device__ __forceinline__ int seq_of(const int* pre, int n_seqs, int id) {
   return lo;
 }
 
-// Block 0 lists the query tiles, block 1 the key tiles.  `at_once`: up to this
-// many entries of the kind start together whatever their order, so they are not
-// sorted; `wide`: the rows they walk over are more than half of L2.
+// Block i makes list i.  `at_once`: up to this many entries of the list start
+// together whatever their order, so they are not sorted; `wide`: the rows that its
+// tiles walk over are more than half of L2.
 struct PlanParams {
-  int n_seqs, total, tt;
-  int cap[2], at_once[2], wide[2];
-  int4* items[2];
-  PackedHeader* head;
+  PackedDims d;
+  PackedPlan plan;
+  int at_once[3], wide[3];
   int* scratch;
   int* status;
 };
@@ -82,10 +81,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   __shared__ int hist[PLAN_CLASSES];
   __shared__ int warp_sums[32];
   __shared__ int longest_s;
-  const int tid = threadIdx.x, kind = blockIdx.x, n_seqs = p.n_seqs;
+  const int tid = threadIdx.x, kind = blockIdx.x, n_seqs = p.d.n_seqs, tt = p.d.tt;
   pdl_launch();
   if (tid == 0) longest_s = 0;
-  const int rows = kind ? 128 : p.tt;  // tokens of a tile
+  const int rows = p.d.rows[kind];  // tokens of a tile
+  const bool keys = kind == LIST_K;
   // The sequences in the order they are taken: first row, length, tiles before it.
   const bool in_smem = n_seqs <= PLAN_SMEM_SEQS;
   int* begin = in_smem ? seq_s : p.scratch + kind * 3 * n_seqs;
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   bool good = true;
   for (int s = tid; s < n_seqs; s += PLAN_THREADS) {
     const int a = cu[s], b = cu[s + 1];
-    good &= a >= 0 && a <= b && b <= p.total;
+    good &= a >= 0 && a <= b && b <= p.d.total;
     if (good) {
       longest = max(longest, b - a);
       most_tiles += (b - a + rows - 1) / rows;
@@ -108,12 +108,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   // output row is then zero) and the status word says so.
   if (!__syncthreads_and(good)) {
     if (tid == 0) {
+      p.plan.head->n[kind] = p.plan.head->next[kind] = 0;
       if (kind == 0) {
         record_error(p.status, KID_PACKED_PLAN, 1);
-        p.head->n_q = 0;
-        p.head->first = p.head->end = 0;
-      } else {
-        p.head->n_k = 0;
+        p.plan.head->first = p.plan.head->end = 0;
       }
     }
     return;
@@ -121,19 +119,16 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   longest = longest_s;
   int n;
   block_scan(most_tiles, warp_sums, &n);
-  const int cap = p.cap[kind];
+  const int cap = p.d.cap[kind];
   if (tid == 0) {
+    p.plan.head->n[kind] = min(n, cap);
+    p.plan.head->next[kind] = 0;
     if (kind == 0) {
-      p.head->n_q = min(n, cap);
-      p.head->first = cu[0];
-      p.head->end = cu[n_seqs];
-    } else {
-      p.head->n_k = min(n, cap);
+      p.plan.head->first = cu[0];
+      p.plan.head->end = cu[n_seqs];
     }
   }
-
-  const int tt = p.tt;
-  const int most = kind ? (longest + tt - 1) / tt : (longest + 127) >> 7;  // steps of the longest tile
+  const int most = keys ? (longest + tt - 1) / tt : (longest + 127) >> 7;  // steps of the longest tile
   const bool by_seq = p.wide[kind] && n >= 8 * max(p.at_once[kind], 1);
   if (!by_seq) {
     for (int s = tid; s < n_seqs; s += PLAN_THREADS) {
@@ -166,7 +161,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
     sum += part;
   }
   __syncthreads();
-  int4* items = p.items[kind];
+  int4* items = p.plan.list[kind];
   auto entry = [&](int id) {
     const int s = seq_of(pre, n_seqs, id);
     return make_int4(begin[s], len[s], by_seq ? pre[s] : id - pre[s], by_seq ? 0 : 1);
@@ -180,8 +175,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   while ((most >> shift) >= PLAN_CLASSES) ++shift;
   auto cls = [&](const int4& e) {
     // steps: key tiles up to the query tile's last token, or query tiles from the key tile's first
-    const int steps = kind ? (e.y + tt - 1) / tt - e.z * 128 / tt
-                           : (int(min((long long)(e.z + 1) * tt, (long long)e.y)) + 127) >> 7;
+    const int steps = keys ? (e.y + tt - 1) / tt - e.z * 128 / tt
+                           : (int(min((long long)(e.z + 1) * rows, (long long)e.y)) + 127) >> 7;
     return (most >> shift) - (steps >> shift);
   };
   hist[tid] = 0;
@@ -236,53 +231,58 @@ int packed_dims(const mea_packed_dims* d, PackedDims* out) {
       o.tt = 128 / p;
     }
   o.hg = d->Hq / o.p;
-  const long long cap_q = (long long)d->total / o.tt + d->n_seqs, cap_k = (long long)d->total / 128 + d->n_seqs;
-  if (cap_q * o.hg > 0x7fffffffLL || cap_k * d->Hkv > 0x7fffffffLL)
-    return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention: total=%d rows, %d sequences and %d heads make too many tiles",
-                     d->total, d->n_seqs, d->Hq);
-  o.cap_q = int(cap_q);
-  o.cap_k = int(cap_k);
+  // Two query tiles to a forward item where that still gives every SM one.
+  o.streams = (long long)d->total / (2 * o.tt) * o.hg >= num_sms() ? 2 : 1;
+  const int rows[3] = {o.tt, 128, o.tt * o.streams}, heads[3] = {o.hg, d->Hkv, o.hg};
+  for (int i = 0; i < 3; ++i) {
+    const long long cap = (long long)d->total / rows[i] + d->n_seqs;
+    if (cap * heads[i] > 0x3fffffffLL)  // (the counters run on by one per SM)
+      return set_error(MEA_ERR_UNSUPPORTED_SHAPE,
+                       "packed attention: total=%d rows, %d sequences and %d heads make too many tiles", d->total,
+                       d->n_seqs, d->Hq);
+    o.rows[i] = rows[i];
+    o.heads[i] = heads[i];
+    o.cap[i] = int(cap);
+  }
   *out = o;
   return MEA_OK;
 }
 
-size_t packed_plan_bytes(const PackedDims& d) {
-  return up256(sizeof(PackedHeader)) + up256(sizeof(int4) * size_t(d.cap_q)) + up256(sizeof(int4) * size_t(d.cap_k)) +
-         (d.n_seqs > PLAN_SMEM_SEQS ? up256(sizeof(int) * 6 * size_t(d.n_seqs)) : 0);
+static size_t plan_scratch(const PackedDims& d) {  // offset of the plan kernel's own space
+  size_t n = up256(sizeof(PackedHeader));
+  for (int i = 0; i < 3; ++i) n += up256(sizeof(int4) * size_t(d.cap[i]));
+  return n;
 }
 
-PackedPlan packed_plan_view(const PackedDims& d, const void* plan) {
-  const char* b = static_cast<const char*>(plan);
+size_t packed_plan_bytes(const PackedDims& d) {
+  return plan_scratch(d) + (d.n_seqs > PLAN_SMEM_SEQS ? up256(sizeof(int) * 9 * size_t(d.n_seqs)) : 0);
+}
+
+PackedPlan packed_plan_view(const PackedDims& d, void* plan) {
+  char* b = static_cast<char*>(plan);
   PackedPlan v;
-  v.head = reinterpret_cast<const PackedHeader*>(b);
+  v.head = reinterpret_cast<PackedHeader*>(b);
   b += up256(sizeof(PackedHeader));
-  v.q_items = reinterpret_cast<const int4*>(b);
-  b += up256(sizeof(int4) * size_t(d.cap_q));
-  v.k_items = reinterpret_cast<const int4*>(b);
+  for (int i = 0; i < 3; ++i) {
+    v.list[i] = reinterpret_cast<int4*>(b);
+    b += up256(sizeof(int4) * size_t(d.cap[i]));
+  }
   return v;
 }
 
 int run_packed_plan(const PackedDims& d, const int* cu, void* plan, int* status, cudaStream_t st) {
-  const PackedPlan v = packed_plan_view(d, plan);
-  char* scratch = static_cast<char*>(plan) + up256(sizeof(PackedHeader)) + up256(sizeof(int4) * size_t(d.cap_q)) +
-                  up256(sizeof(int4) * size_t(d.cap_k));
   PlanParams p;
-  p.n_seqs = d.n_seqs;
-  p.total = d.total;
-  p.tt = d.tt;
-  p.cap[0] = d.cap_q;
-  p.cap[1] = d.cap_k;
-  p.at_once[0] = num_sms() / d.hg;  // times hg head groups: one CTA an SM in the dQ kernel
-  p.at_once[1] = num_sms() / d.Hkv;
+  p.d = d;
+  p.plan = packed_plan_view(d, plan);
   constexpr long long kHalfL2 = 64LL << 20;
-  p.wide[0] = 4LL * d.total * d.Hkv * d.N > kHalfL2;  // K and V
-  p.wide[1] = 4LL * d.total * d.Hq * d.N > kHalfL2;   // Q and dO
-  p.items[0] = const_cast<int4*>(v.q_items);
-  p.items[1] = const_cast<int4*>(v.k_items);
-  p.head = const_cast<PackedHeader*>(v.head);
-  p.scratch = reinterpret_cast<int*>(scratch);
+  const bool wide_kv = 4LL * d.total * d.Hkv * d.N > kHalfL2, wide_q = 4LL * d.total * d.Hq * d.N > kHalfL2;
+  for (int i = 0; i < 3; ++i) {
+    p.at_once[i] = num_sms() / d.heads[i];
+    p.wide[i] = i == LIST_K ? wide_q : wide_kv;  // Q and dO, or K and V
+  }
+  p.scratch = reinterpret_cast<int*>(static_cast<char*>(plan) + plan_scratch(d));
   p.status = status;
-  packed_plan_kernel<<<2, PLAN_THREADS, 0, st>>>(cu, p);
+  packed_plan_kernel<<<3, PLAN_THREADS, 0, st>>>(cu, p);
   return check_launch("packed_plan_kernel");
 }
 
