@@ -144,6 +144,49 @@ struct PackedTile {
   }
 };
 
+// 64 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_load64(uint32_t taddr, float2 (&v)[32]) {
+  uint32_t a[32], b[32];
+  tmem_ld32(taddr, a);
+  tmem_ld32(taddr + 32, b);
+  tmem_wait_ld_tied2x32(a, b);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    v[e] = make_float2(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]));
+    v[16 + e] = make_float2(__uint_as_float(b[2 * e]), __uint_as_float(b[2 * e + 1]));
+  }
+}
+
+// A warp's 32 rows to global memory, 32 columns at a time through 2 KB of shared
+// memory: with one row per lane a store instruction would touch 32 rows (and take
+// as many passes), this way it writes 64 bytes of each of eight.
+struct WarpRows {
+  static constexpr uint32_t BYTES = 2048;
+  uint32_t buf;
+  int lane;
+  int off[4];    // element offsets of rows lane / 4 + 8 i
+  bool live[4];  // rows to be written
+  // Columns [col, col + 32) of this lane's row times `scale`, n columns in all.
+  template <class T>
+  __device__ __forceinline__ void store32(const float2* v, float scale, uint16_t* out, int col, int n) const {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      sts128(buf + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4), T::pack(v[4 * u].x * scale, v[4 * u].y * scale),
+             T::pack(v[4 * u + 1].x * scale, v[4 * u + 1].y * scale), T::pack(v[4 * u + 2].x * scale, v[4 * u + 2].y * scale),
+             T::pack(v[4 * u + 3].x * scale, v[4 * u + 3].y * scale));
+    __syncwarp();
+    const int unit = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (lane >> 2) + 8 * i;
+      uint32_t w[4];
+      lds128(buf + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4), w);
+      if (live[i] && col + 8 * unit < n) st_global_v4(out + off[i] + col + 8 * unit, w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+  }
+};
+
 // Rows of `width` 16-byte units outside [first, end) of a [total, width] output
 // to zero, spread over the grid: no sequence owns them.
 __device__ __forceinline__ void zero_outside(uint4* out, int total, int first, int end, long long width, int block,

@@ -21,6 +21,8 @@
 // Warps (384 threads, persistent, one CTA per SM): 0 TMA, 1 MMA issue, 2 (dK/dV)
 // lse2 and delta rows, 4..11 softmax: two warps per TMEM lane quarter, half a row
 // each.
+#include <type_traits>
+
 #include "attn_packed.h"
 #include "attn_packed.cuh"
 
@@ -85,32 +87,17 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, PackedH
 }
 
 // ---------------------------------------------------------------- common
-// 32 columns of this thread's TMEM lane times `scale` to 16-bit values at out[c], c < n_left.
-template <class T>
-__device__ __forceinline__ void store_cols32(uint32_t taddr, float scale, uint16_t* out, int n_left, bool live) {
-  uint32_t v[32];
-  __syncwarp();
-  tmem_load32(taddr, v);
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = T::pack(__uint_as_float(v[8 * u + 2 * e]) * scale, __uint_as_float(v[8 * u + 2 * e + 1]) * scale);
-    if (live && 8 * u < n_left) st_global_v4(out + 8 * u, w[0], w[1], w[2], w[3]);
-  }
-}
-
 // ---------------------------------------------------------------- dQ
 template <int HD>
 struct PackedDqCfg {
   static constexpr int QB = HD <= 64 ? 2 : 1;  // Q/dO buffers: the next item's load overlaps this one
   static constexpr int KS = 2, VS = 2;
   static constexpr uint32_t TB = 128 * HD * 2;
-  static constexpr uint32_t S_COL = 0, DP_COL = 128, DS_COL = 256, DQ_COL = 320;
+  static constexpr uint32_t S_COL = 0, DP_COL = 128, DS_COL = 256, DQ_COL = 384;  // two dS buffers
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
-  static constexpr size_t SMEM = 1024 + OFF_BAR + 512;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows::BYTES;
 };
 
 struct DqItem {
@@ -155,11 +142,12 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
   auto v_empty = [&](int s) { return b0 + 8u * (10 + s); };
   const uint32_t s_full = b0 + 8u * 12, s_empty = b0 + 8u * 13;    // S computed / read by the softmax
   const uint32_t dp_full = b0 + 8u * 14, dp_empty = b0 + 8u * 15;  // dP the same
-  const uint32_t ds_full = b0 + 8u * 16, ds_free = b0 + 8u * 17;   // dS written / read by the dQ MMAs
-  const uint32_t dq_full = b0 + 8u * 18, dq_empty = b0 + 8u * 19;  // an item's dQ complete / read out
-  const uint32_t k_raw = b0 + 8u * 20, drain_bar = b0 + 8u * 21;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
-  const Feed feed{b0 + 8u * 22, b0 + 8u * 26, reinterpret_cast<int*>(bars + 31)};
+  const uint32_t ds_full = b0 + 8u * 16;                           // dS written
+  auto ds_free = [&](int b) { return b0 + 8u * (17 + b); };        // read by the dQ MMAs, per buffer
+  const uint32_t dq_full = b0 + 8u * 19, dq_empty = b0 + 8u * 20;  // an item's dQ complete / read out
+  const uint32_t k_raw = b0 + 8u * 21, drain_bar = b0 + 8u * 22;
+  const Feed feed{b0 + 8u * 23, b0 + 8u * 27, reinterpret_cast<int*>(bars + 31)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -170,7 +158,8 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     mbar_init(dp_full, 1);
     mbar_init(dp_empty, 256);
     mbar_init(ds_full, 256);
-    mbar_init(ds_free, 1);
+    mbar_init(ds_free(0), 1);
+    mbar_init(ds_free(1), 1);
     mbar_init(dq_full, 1);
     mbar_init(dq_empty, 256);
     mbar_init(k_raw, 1);
@@ -329,22 +318,20 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           const bool more = nkv1 > 0;
           if (j + 1 == nkv) nkv_next = nkv1;  // the lookahead stands at the next item by now
           // With one Q/dO buffer the next item's rows arrive late: this item's last dQ goes first.
-          const bool late = QB == 1 && j + 1 == nkv;
-          auto ahead = [&]() -> bool {
-            return mbar_wait(s_empty, n & 1, g, 11) && issue_s() && mbar_wait(dp_empty, n & 1, g, 12) && issue_dp();
-          };
-          if (more && !late && !ahead()) break;
+          const bool early = more && (QB == 2 || j + 1 < nkv);
+          if (early && !(mbar_wait(s_empty, n & 1, g, 11) && issue_s())) break;
           if (!mbar_wait(ds_full, n & 1, g, 13)) break;
           if (j == 0 && item > 0 && !mbar_wait(dq_empty, (item - 1) & 1, g, 14)) break;
           tc_fence_after();
 #pragma unroll
           for (int kc = 0; kc < 8; ++kc)
-            mma_ts(tmem + Cfg::DQ_COL, tmem + Cfg::DS_COL + kc * 8, Tile::mnmajor(sK(sk), 128, kc), IDESC_DQ,
+            mma_ts(tmem + Cfg::DQ_COL, tmem + Cfg::DS_COL + 64 * (n & 1) + kc * 8, Tile::mnmajor(sK(sk), 128, kc), IDESC_DQ,
                    (j > 0 || kc > 0) ? 1u : 0u);
           mma_commit(k_empty(sk));
-          mma_commit(ds_free);
+          mma_commit(ds_free(n & 1));
           if (j + 1 == nkv) mma_commit(dq_full);
-          if (more && late && !ahead()) break;
+          if (more && !early && !(mbar_wait(s_empty, n & 1, g, 11) && issue_s())) break;
+          if (more && !(mbar_wait(dp_empty, n & 1, g, 12) && issue_dp())) break;
         }
         nkv = nkv_next;
         ++item;
@@ -361,6 +348,14 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     const int tok = r / p.d.p, hr = r - tok * p.d.p;
+    WarpRows out{base + Cfg::OFF_OUT + (warp - 4) * WarpRows::BYTES, lane};
+    int out_tok[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = quarter * 32 + (lane >> 2) + 8 * i;
+      out_tok[i] = row / p.d.p;
+      out.off[i] = (out_tok[i] * p.d.Hq + row - out_tok[i] * p.d.p) * p.d.N;
+    }
     bool ok = true;
     int n = 0, item = 0;
     while (ok) {
@@ -381,55 +376,71 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
         const bool mask = 128 * j + 127 > w.t0;
         const int cmax = t - 128 * j - 64 * hh;  // last of this thread's columns that the row sees
         float2 P[32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t a[16];
-          tmem_load16(lane_base + Cfg::S_COL + 64 * hh + 16 * c, a);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            P[8 * c + e] = exp2_pair(ffma2(make_float2(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1])), sl2, neg_lse),
-                                     (kPolyPairsBwd >> e) & 1);
-        }
+        tmem_load64(lane_base + Cfg::S_COL + 64 * hh, P);
         tc_fence_before();
-        mbar_arrive(s_empty);
+        mbar_arrive(s_empty);  // the scores are in registers
+#pragma unroll
+        for (int e = 0; e < 32; ++e) P[e] = exp2_pair(ffma2(P[e], sl2, neg_lse), (kPolyPairsBwd >> (e & 7)) & 1);
         ok = __all_sync(0xffffffffu, mbar_wait(dp_full, n & 1, g, 16));
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (n - 1) & 1, g, 17));
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t a[16], ds[8];
-          tmem_load16(lane_base + Cfg::DP_COL + 64 * hh + 16 * c, a);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float2 s = fmul2(P[8 * c + e], fsub2(make_float2(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1])), dl2));
-            if (mask) {
-              s.x = 16 * c + 2 * e > cmax ? 0.f : s.x;
-              s.y = 16 * c + 2 * e + 1 > cmax ? 0.f : s.y;
-            }
-            ds[e] = T::pack(s.x, s.y);
-          }
-          tmem_st8(lane_base + Cfg::DS_COL + 32 * hh + 8 * c, ds);
-        }
-        tmem_st_wait();
+        float2 dp[32];
+        tmem_load64(lane_base + Cfg::DP_COL + 64 * hh, dp);
         tc_fence_before();
         mbar_arrive(dp_empty);
+        if (n > 1) {
+          ok = __all_sync(0xffffffffu, mbar_wait(ds_free(n & 1), ((n >> 1) - 1) & 1, g, 17));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        auto grad = [&](auto masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t ds[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float2 s = fmul2(P[8 * c + e], fsub2(dp[8 * c + e], dl2));
+              if (masked()) {
+                s.x = 16 * c + 2 * e > cmax ? 0.f : s.x;
+                s.y = 16 * c + 2 * e + 1 > cmax ? 0.f : s.y;
+              }
+              ds[e] = T::pack(s.x, s.y);
+            }
+            tmem_st8(lane_base + Cfg::DS_COL + 64 * (n & 1) + 32 * hh + 8 * c, ds);
+          }
+        };
+        if (mask)
+          grad(std::true_type());
+        else
+          grad(std::false_type());
+        tmem_st_wait();
+        tc_fence_before();
         mbar_arrive(ds_full);
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, mbar_wait(dq_full, item & 1, g, 18));
       if (!ok) break;
       tc_fence_after();
-      const int col = hh * (HD / 2);
+      float2 dq[HD / 4];
+      if constexpr (HD == 128) {
+        tmem_load64(lane_base + Cfg::DQ_COL + 64 * hh, *reinterpret_cast<float2(*)[32]>(dq));
+      } else {
+        uint32_t v[32];
+        tmem_load32(lane_base + Cfg::DQ_COL + 32 * hh, v);
 #pragma unroll
-      for (int c = 0; c < HD / 2; c += 32)
-        store_cols32<T>(lane_base + Cfg::DQ_COL + col + c, p.scale, p.dq + row * p.d.N + col + c, p.d.N - col - c, live);
+        for (int e = 0; e < 16; ++e) dq[e] = make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+      }
       tc_fence_before();
       mbar_arrive(dq_empty);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out.live[i] = out_tok[i] < w.t1 - w.t0;
+      uint16_t* tile = p.dq + ((long long)(w.seq0 + w.t0) * p.d.Hq + w.h0) * p.d.N;
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) out.store32<T>(dq + 16 * c, p.scale, tile, hh * (HD / 2) + 32 * c, p.d.N);
       ++item;
     }
-    // The last step's ds_free has landed before this CTA's shared memory goes away.
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (n - 1) & 1, g, 19));
+    // The last two steps' ds_free have landed before this CTA's shared memory goes away.
+    for (int m = n > 1 ? n - 2 : 0; ok && m < n; ++m) ok = __all_sync(0xffffffffu, mbar_wait(ds_free(m & 1), (m >> 1) & 1, g, 19));
     if (!ok) g.ok = false;
   }
 
@@ -452,7 +463,8 @@ struct PackedDkvCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static_assert(DK_COL + HD <= 512, "TMEM budget");
   static constexpr uint32_t OFF_Q = KVB * 2 * TB, OFF_ROW = OFF_Q + ST * 2 * TB, OFF_BAR = OFF_ROW + ST * 1024;
-  static constexpr size_t SMEM = 1024 + OFF_BAR + 512;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows::BYTES;
 };
 
 struct DkvItem {
@@ -692,7 +704,9 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           for (int kc = 0; kc < 8; ++kc)
             mma_ts(tmem + Cfg::DV_COL, pt + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sdO(s), 128, kc), IDESC_KV,
                    (k > 0 || kc > 0) ? 1u : 0u);
-          if (SB == 1 && as.left && !issue_s()) break;
+          // One buffer: after dV, or after the item's last dK, which should not wait for the next K and V.
+          const bool last = k + 1 == steps;
+          if (SB == 1 && as.left && !last && !issue_s()) break;
           if (!mbar_wait(ds_full, n & 1, g, 10)) break;
           tc_fence_after();
           // dK += dS^T Q
@@ -701,7 +715,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             mma_ts(tmem + Cfg::DK_COL, dst + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sQ(s), 128, kc), IDESC_KV,
                    (k > 0 || kc > 0) ? 1u : 0u);
           mma_commit(qdo_empty(s));
-          if (k + 1 == steps) mma_commit(acc_full);
+          if (last) mma_commit(acc_full);
+          if (SB == 1 && as.left && last && !issue_s()) break;
           if (ad.left) issue_dp();
         }
       }
@@ -740,6 +755,9 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+    WarpRows out{base + Cfg::OFF_OUT + (warp - 4) * WarpRows::BYTES, lane};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out.off[i] = (quarter * 32 + (lane >> 2) + 8 * i) * p.d.Hkv * p.d.N;
     bool ok = true;
     int n = 0, item = 0;
     while (ok) {
@@ -763,50 +781,51 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           const uint32_t sa = lane_base + Cfg::S_COL + 128 * (n % SB) + 64 * hh;
           const uint32_t da = lane_base + Cfg::DP_COL + 64 * hh;
           float2 P[32];
+          tmem_load64(sa, P);
+          auto probs = [&](auto masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t a[16], pk[8];
-            tmem_load16(sa + 16 * c, a);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t pk[8];
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float4 l = lse4[4 * c + (e >> 1)];
+              for (int e = 0; e < 8; e += 2) {
+                const float4 l = lse4[4 * c + (e >> 1)];
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                float2 x = exp2_pair(ffma2(make_float2(__uint_as_float(a[2 * (e + u)]), __uint_as_float(a[2 * (e + u) + 1])),
-                                           sl2, u ? make_float2(l.z, l.w) : make_float2(l.x, l.y)),
-                                     (kPolyPairsBwd >> (e + u)) & 1);
-                if (mask) {
-                  x.x = 16 * c + 2 * (e + u) < cmin ? 0.f : x.x;
-                  x.y = 16 * c + 2 * (e + u) + 1 < cmin ? 0.f : x.y;
+                for (int u = 0; u < 2; ++u) {
+                  float2 x = exp2_pair(ffma2(P[8 * c + e + u], sl2, u ? make_float2(l.z, l.w) : make_float2(l.x, l.y)),
+                                       (kPolyPairsBwd >> (e + u)) & 1);
+                  if (masked()) {
+                    x.x = 16 * c + 2 * (e + u) < cmin ? 0.f : x.x;
+                    x.y = 16 * c + 2 * (e + u) + 1 < cmin ? 0.f : x.y;
+                  }
+                  P[8 * c + e + u] = x;
+                  pk[e + u] = T::pack(x.x, x.y);
                 }
-                P[8 * c + e + u] = x;
-                pk[e + u] = T::pack(x.x, x.y);
               }
+              tmem_st8(sa + 8 * c, pk);  // over columns this thread has read
             }
-            tmem_st8(sa + 8 * c, pk);  // over columns this thread has read
-          }
+          };
+          if (mask)
+            probs(std::true_type());
+          else
+            probs(std::false_type());
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(p_full(n % SB));
           ok = __all_sync(0xffffffffu, mbar_wait(dp_full, n & 1, g, 14));
           if (!ok) break;
           tc_fence_after();
+          float2 dp[32];
+          tmem_load64(da, dp);
+          // (Masked entries have P = 0; keys of other sequences are other lanes, their rows of dO are cleared.)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t a[16], ds[8];
-            tmem_load16(da + 16 * c, a);
+            uint32_t ds[8];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
               const float4 l = dl4[4 * c + (e >> 1)];
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                float2 x = fmul2(P[8 * c + e + u],
-                                 fsub2(make_float2(__uint_as_float(a[2 * (e + u)]), __uint_as_float(a[2 * (e + u) + 1])),
-                                       u ? make_float2(l.z, l.w) : make_float2(l.x, l.y)));
-                if (mask) {
-                  x.x = 16 * c + 2 * (e + u) < cmin ? 0.f : x.x;
-                  x.y = 16 * c + 2 * (e + u) + 1 < cmin ? 0.f : x.y;
-                }
+                const float2 x = fmul2(P[8 * c + e + u], fsub2(dp[8 * c + e + u], u ? make_float2(l.z, l.w) : make_float2(l.x, l.y)));
                 ds[e + u] = T::pack(x.x, x.y);
               }
             }
@@ -821,13 +840,22 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       if (!ok) break;
       tc_fence_after();
       // Warps 4..7 write dV, 8..11 dK.
-      uint16_t* out = (hh ? p.dk : p.dv) + ((long long)(w.seq0 + key) * p.d.Hkv + w.kvh) * p.d.N;
+      uint16_t* tile = (hh ? p.dk : p.dv) + ((long long)(w.seq0 + w.k0) * p.d.Hkv + w.kvh) * p.d.N;
       const uint32_t acc = lane_base + (hh ? Cfg::DK_COL : Cfg::DV_COL);
       const float sc = hh ? p.scale : 1.0f;
 #pragma unroll
-      for (int c = 0; c < HD; c += 32) store_cols32<T>(acc + c, sc, out + c, p.d.N - c, key < w.len);
-      tc_fence_before();
-      mbar_arrive(acc_empty);
+      for (int i = 0; i < 4; ++i) out.live[i] = w.k0 + quarter * 32 + (lane >> 2) + 8 * i < w.len;
+#pragma unroll
+      for (int c = 0; c < HD; c += 64) {
+        float2 v[32];
+        tmem_load64(acc + c, v);
+        if (c + 64 == HD) {
+          tc_fence_before();
+          mbar_arrive(acc_empty);
+        }
+        out.store32<T>(v, sc, tile, c, p.d.N);
+        out.store32<T>(v + 16, sc, tile, c + 32, p.d.N);
+      }
       ++item;
     }
     if (!ok) g.ok = false;

@@ -50,7 +50,8 @@ struct PackedFwdCfg {
   static constexpr uint32_t O_COL = SEP_P ? 384 : 256;
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
-  static constexpr size_t SMEM = 1024 + OFF_BAR + 512;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows::BYTES;
   static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 };
 
@@ -359,6 +360,14 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
     const uint32_t st = lane_base + Cfg::S_COL + 128 * x, pt = lane_base + Cfg::P_COL + Cfg::P_STEP * x;
     const uint32_t ot = lane_base + Cfg::O_COL + HD * x;
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+    WarpRows out{base + Cfg::OFF_OUT + (warp - 4) * WarpRows::BYTES, lane};
+    int out_tok[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (warp & 3) * 32 + (lane >> 2) + 8 * i;
+      out_tok[i] = row / p.d.p;
+      out.off[i] = (out_tok[i] * p.d.Hq + row - out_tok[i] * p.d.p) * p.d.N;
+    }
     bool ok = true;
     int n = 0, outs = 0;  // steps and items of this stream
     for (int item = 0; ok; ++item) {
@@ -477,45 +486,32 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
       if (!ok) break;
       tc_fence_after();
       ++outs;
-      float f[HD];
+      float2 f[HD / 2];
 #pragma unroll
-      for (int c = 0; c < HD; c += 64) {
-        uint32_t a[32], b[32];
-        tmem_ld32(ot + c, a);
-        tmem_ld32(ot + c + 32, b);
-        tmem_wait_ld_tied2x32(a, b);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          f[c + e] = __uint_as_float(a[e]);
-          f[c + 32 + e] = __uint_as_float(b[e]);
-        }
-      }
+      for (int c = 0; c < HD / 64; ++c) tmem_load64(ot + 64 * c, *reinterpret_cast<float2(*)[32]>(f + 32 * c));
       tc_fence_before();
       mbar_arrive(o_empty(x));
       nan_row |= m_run == -INFINITY;  // no finite score: 0 / 0
       const float inv_l = nan_row ? __int_as_float(0x7fffffff) : 1.0f / l_run;
-#pragma unroll
-      for (int e = 0; e < HD; ++e) f[e] *= inv_l;
       if (bad[(item & 3) * 2 + x] && live) {  // the inf and NaN elements that were cleared, for the rows that see them
 #pragma unroll 1
         for (int key = w.t0 + 1; key <= t; ++key) {
           const uint16_t* vr = static_cast<const uint16_t*>(p.v) + (long long)(w.seq0 + key) * p.v_tok + w.kvh * p.v_head;
 #pragma unroll
-          for (int e = 0; e < HD; ++e)
-            if (e < p.d.N && half_nonfinite<T>(vr[e])) f[e] += T::lo(vr[e]);
+          for (int e = 0; e < HD / 2; ++e) {
+            if (2 * e < p.d.N && half_nonfinite<T>(vr[2 * e])) f[e].x += T::lo(vr[2 * e]);
+            if (2 * e < p.d.N && half_nonfinite<T>(vr[2 * e + 1])) f[e].y += T::lo(vr[2 * e + 1]);
+          }
         }
       }
-      const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
-      if (live) {
-        uint16_t* orow = static_cast<uint16_t*>(p.o) + row * p.d.N;
-#pragma unroll
-        for (int c = 0; c < HD; c += 8)
-          if (c < p.d.N)
-            st_global_v4(orow + c, T::pack(f[c], f[c + 1]), T::pack(f[c + 2], f[c + 3]), T::pack(f[c + 4], f[c + 5]),
-                         T::pack(f[c + 6], f[c + 7]));
-        p.lse2[row] = nan_row ? __int_as_float(0x7fffffff) : m_run + __log2f(l_run);
-      }
       __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out.live[i] = out_tok[i] < min(p.d.tt, w.end - first);
+      uint16_t* tile = static_cast<uint16_t*>(p.o) + ((long long)(w.seq0 + first) * p.d.Hq + w.h0) * p.d.N;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) out.store32<T>(f + 16 * c, inv_l, tile, 32 * c, p.d.N);
+      const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
+      if (live) p.lse2[row] = nan_row ? __int_as_float(0x7fffffff) : m_run + __log2f(l_run);
     }
     // The last pv_done has landed before this CTA's shared memory goes away.
     if (Cfg::SEP_P && ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done(x), (n - 1) & 1, g, 18));

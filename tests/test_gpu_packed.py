@@ -154,6 +154,28 @@ def test_causal_whatever_later_rows_hold(n, hq, hkv, value):
     assert not bool(torch.isfinite(got[90:200, :, 5]).any())
 
 
+@pytest.mark.parametrize("value", [float("nan"), -float("inf")])
+@pytest.mark.parametrize("hq,hkv,n", [(16, 16, 64), (12, 12, 128), (40, 5, 64)])
+def test_causal_with_two_tiles_to_an_item(hq, hkv, n, value):
+    """Enough rows that the forward takes two query tiles at a time: v elements behind each of several cut points hold
+    inf or NaN, inside either tile of a pair and at their border."""
+    lens = [2000, 1111, 889]
+    q, k, v, do, cu = _make(lens, hq, hkv, n, BF, seed=13)
+    cut = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    clean = packed_attention(q, k, v, cut)
+    tt = 128 // (hq // hkv)
+    for at in (1, tt - 1, tt, tt + 1, 2 * tt, 1000, 1999):
+        v2 = v.clone()
+        v2[at, :, 3] = value
+        got = packed_attention(q, k, v2, cut)
+        assert torch.equal(got[:at], clean[:at]) and torch.equal(got[2000:], clean[2000:]), at
+        assert not bool(torch.isfinite(got[at:2000, :, 3]).any()), at
+        k2 = k.clone()
+        k2[at:2000] = value
+        got = packed_attention(q, k2, v, cut)
+        assert torch.equal(got[:at], clean[:at]) and torch.equal(got[2000:], clean[2000:]), at
+
+
 def test_nan_query_row_is_nan():
     q, k, v, do, cu = _make([140], 2, 1, 64, BF, seed=13)
     cut = torch.tensor(cu, dtype=torch.int32, device=DEV)
