@@ -97,7 +97,7 @@ struct PackedDqCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<HD>::BYTES;
 };
 
 struct DqItem {
@@ -348,13 +348,12 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     const int tok = r / p.d.p, hr = r - tok * p.d.p;
-    WarpRows out{base + Cfg::OFF_OUT + (warp - 4) * WarpRows::BYTES, lane};
+    WarpRows<HD> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<HD>::BYTES, lane, quarter * 32);
     int out_tok[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = quarter * 32 + (lane >> 2) + 8 * i;
-      out_tok[i] = row / p.d.p;
-      out.off[i] = (out_tok[i] * p.d.Hq + row - out_tok[i] * p.d.p) * p.d.N;
+    for (int i = 0; i < out.rows(); ++i) {
+      out_tok[i] = out.row(i) / p.d.p;
+      out.off[i] = (out_tok[i] * p.d.Hq + out.row(i) - out_tok[i] * p.d.p) * p.d.N;
     }
     bool ok = true;
     int n = 0, item = 0;
@@ -433,10 +432,10 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
       tc_fence_before();
       mbar_arrive(dq_empty);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out.live[i] = out_tok[i] < w.t1 - w.t0;
+      for (int i = 0; i < out.rows(); ++i) out.live[i] = out_tok[i] < w.t1 - w.t0;
       uint16_t* tile = p.dq + ((long long)(w.seq0 + w.t0) * p.d.Hq + w.h0) * p.d.N;
 #pragma unroll
-      for (int c = 0; c < HD / 64; ++c) out.store32<T>(dq + 16 * c, p.scale, tile, hh * (HD / 2) + 32 * c, p.d.N);
+      for (int c = 0; c < HD / 64; ++c) out.template store32<T>(dq + 16 * c, p.scale, tile, hh * (HD / 2) + 32 * c, p.d.N);
       ++item;
     }
     // The last two steps' ds_free have landed before this CTA's shared memory goes away.
@@ -461,10 +460,11 @@ struct PackedDkvCfg {
   static constexpr uint32_t TB = 128 * HD * 2;
   static constexpr uint32_t S_COL = 0, DP_COL = SB * 128, DV_COL = DP_COL + 128, DK_COL = DV_COL + HD;
   static constexpr uint32_t TMEM_COLS = 512;
+  static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
   static_assert(DK_COL + HD <= 512, "TMEM budget");
   static constexpr uint32_t OFF_Q = KVB * 2 * TB, OFF_ROW = OFF_Q + ST * 2 * TB, OFF_BAR = OFF_ROW + ST * 1024;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<HD>::BYTES;
 };
 
 struct DkvItem {
@@ -561,6 +561,16 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   const int n_items = p.plan.head->n[LIST_K] * p.d.Hkv;
   Guard g(p.status, KID_PACKED_DKV);
 
+  auto finish = [&]() {  // TMEM is freed once every warp is done with it
+    tc_fence_before();
+    named_bar_sync(1, 384);
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, Cfg::TMEM_COLS);
+    }
+  };
+  if (warp < 4) {
+  reg_dealloc<Cfg::REG_REST>();
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     const bool lead = lane == 0;
@@ -749,15 +759,20 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           mbar_arrive(row_full(s));
         }
     }
-  } else if (warp >= 4) {
+  }
+  finish();
+  return;
+  }
+  reg_alloc<Cfg::REG_SOFTMAX>();
+  {
     // ---------------- softmax warps 4..11: key row r, queries [64 hh, 64 hh + 64) ----------------
     const int quarter = warp & 3, hh = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    WarpRows out{base + Cfg::OFF_OUT + (warp - 4) * WarpRows::BYTES, lane};
+    WarpRows<HD> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<HD>::BYTES, lane, quarter * 32);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out.off[i] = (quarter * 32 + (lane >> 2) + 8 * i) * p.d.Hkv * p.d.N;
+    for (int i = 0; i < out.rows(); ++i) out.off[i] = out.row(i) * p.d.Hkv * p.d.N;
     bool ok = true;
     int n = 0, item = 0;
     while (ok) {
@@ -770,36 +785,44 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
         for (int qt = w.qt0; qt < w.nqt; ++qt, ++n) {
           const int s = n % ST;
           ok = __all_sync(0xffffffffu, mbar_wait(row_full(s), (n / ST) & 1, g, 12));
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full(n % SB), (n / SB) & 1, g, 13));
           if (!ok) break;
-          tc_fence_after();
           const int t0 = qt * p.d.tt;
           const bool mask = t0 < w.k0 + 127;
           const int cmin = p.d.p * (key - t0) - 64 * hh;  // first of this thread's columns that sees the key
-          const float4* lse4 = reinterpret_cast<const float4*>(rows + s * 256 + 64 * hh);
-          const float4* dl4 = reinterpret_cast<const float4*>(rows + s * 256 + 128 + 64 * hh);
           const uint32_t sa = lane_base + Cfg::S_COL + 128 * (n % SB) + 64 * hh;
           const uint32_t da = lane_base + Cfg::DP_COL + 64 * hh;
-          float2 P[32];
+          // The columns' -lse2 and, below, delta come to registers before the waits for
+          // S^T and dP^T: shared memory is busy with the MMAs' operands then.
+          auto row_values = [&](int which, float2(&v)[32]) {
+            const float4* q = reinterpret_cast<const float4*>(rows + s * 256 + 128 * which + 64 * hh);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float4 f = q[e];
+              v[2 * e] = make_float2(f.x, f.y);
+              v[2 * e + 1] = make_float2(f.z, f.w);
+            }
+          };
+          float2 P[32], rv[32];
+          row_values(0, rv);
+          ok = __all_sync(0xffffffffu, mbar_wait(s_full(n % SB), (n / SB) & 1, g, 13));
+          if (!ok) break;
+          tc_fence_after();
           tmem_load64(sa, P);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) P[e] = ffma2(P[e], sl2, rv[e]);
           auto probs = [&](auto masked) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t pk[8];
 #pragma unroll
-              for (int e = 0; e < 8; e += 2) {
-                const float4 l = lse4[4 * c + (e >> 1)];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  float2 x = exp2_pair(ffma2(P[8 * c + e + u], sl2, u ? make_float2(l.z, l.w) : make_float2(l.x, l.y)),
-                                       (kPolyPairsBwd >> (e + u)) & 1);
-                  if (masked()) {
-                    x.x = 16 * c + 2 * (e + u) < cmin ? 0.f : x.x;
-                    x.y = 16 * c + 2 * (e + u) + 1 < cmin ? 0.f : x.y;
-                  }
-                  P[8 * c + e + u] = x;
-                  pk[e + u] = T::pack(x.x, x.y);
+              for (int e = 0; e < 8; ++e) {
+                float2 x = exp2_pair(P[8 * c + e], (kPolyPairsBwd >> e) & 1);
+                if (masked()) {
+                  x.x = 16 * c + 2 * e < cmin ? 0.f : x.x;
+                  x.y = 16 * c + 2 * e + 1 < cmin ? 0.f : x.y;
                 }
+                P[8 * c + e] = x;
+                pk[e] = T::pack(x.x, x.y);
               }
               tmem_st8(sa + 8 * c, pk);  // over columns this thread has read
             }
@@ -811,25 +834,22 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(p_full(n % SB));
+          row_values(1, rv);
           ok = __all_sync(0xffffffffu, mbar_wait(dp_full, n & 1, g, 14));
           if (!ok) break;
           tc_fence_after();
-          float2 dp[32];
-          tmem_load64(da, dp);
           // (Masked entries have P = 0; keys of other sequences are other lanes, their rows of dO are cleared.)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t ds[8];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t dp[32], ds[16];
+            tmem_load32(da + 32 * h, dp);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float4 l = dl4[4 * c + (e >> 1)];
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const float2 x = fmul2(P[8 * c + e + u], fsub2(dp[8 * c + e + u], u ? make_float2(l.z, l.w) : make_float2(l.x, l.y)));
-                ds[e + u] = T::pack(x.x, x.y);
-              }
+            for (int e = 0; e < 16; ++e) {
+              const float2 x = fmul2(P[16 * h + e], fsub2(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])),
+                                                          rv[16 * h + e]));
+              ds[e] = T::pack(x.x, x.y);
             }
-            tmem_st8(da + 8 * c, ds);
+            tmem_st16(da + 16 * h, ds);
           }
           tmem_st_wait();
           tc_fence_before();
@@ -844,7 +864,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       const uint32_t acc = lane_base + (hh ? Cfg::DK_COL : Cfg::DV_COL);
       const float sc = hh ? p.scale : 1.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out.live[i] = w.k0 + quarter * 32 + (lane >> 2) + 8 * i < w.len;
+      for (int i = 0; i < out.rows(); ++i) out.live[i] = w.k0 + out.row(i) < w.len;
 #pragma unroll
       for (int c = 0; c < HD; c += 64) {
         float2 v[32];
@@ -853,19 +873,13 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           tc_fence_before();
           mbar_arrive(acc_empty);
         }
-        out.store32<T>(v, sc, tile, c, p.d.N);
-        out.store32<T>(v + 16, sc, tile, c + 32, p.d.N);
+        out.template store32<T>(v, sc, tile, c, p.d.N);
+        out.template store32<T>(v + 16, sc, tile, c + 32, p.d.N);
       }
       ++item;
     }
     if (!ok) g.ok = false;
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, Cfg::TMEM_COLS);
+    finish();
   }
 }
 

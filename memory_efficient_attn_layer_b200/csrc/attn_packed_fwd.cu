@@ -51,7 +51,7 @@ struct PackedFwdCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<HD>::BYTES;
   static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 };
 
@@ -360,13 +360,12 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
     const uint32_t st = lane_base + Cfg::S_COL + 128 * x, pt = lane_base + Cfg::P_COL + Cfg::P_STEP * x;
     const uint32_t ot = lane_base + Cfg::O_COL + HD * x;
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    WarpRows out{base + Cfg::OFF_OUT + (warp - 4) * WarpRows::BYTES, lane};
+    WarpRows<HD> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<HD>::BYTES, lane, (warp & 3) * 32);
     int out_tok[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = (warp & 3) * 32 + (lane >> 2) + 8 * i;
-      out_tok[i] = row / p.d.p;
-      out.off[i] = (out_tok[i] * p.d.Hq + row - out_tok[i] * p.d.p) * p.d.N;
+    for (int i = 0; i < out.rows(); ++i) {
+      out_tok[i] = out.row(i) / p.d.p;
+      out.off[i] = (out_tok[i] * p.d.Hq + out.row(i) - out_tok[i] * p.d.p) * p.d.N;
     }
     bool ok = true;
     int n = 0, outs = 0;  // steps and items of this stream
@@ -506,10 +505,10 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
       }
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out.live[i] = out_tok[i] < min(p.d.tt, w.end - first);
+      for (int i = 0; i < out.rows(); ++i) out.live[i] = out_tok[i] < min(p.d.tt, w.end - first);
       uint16_t* tile = static_cast<uint16_t*>(p.o) + ((long long)(w.seq0 + first) * p.d.Hq + w.h0) * p.d.N;
 #pragma unroll
-      for (int c = 0; c < HD / 32; ++c) out.store32<T>(f + 16 * c, inv_l, tile, 32 * c, p.d.N);
+      for (int c = 0; c < HD / 32; ++c) out.template store32<T>(f + 16 * c, inv_l, tile, 32 * c, p.d.N);
       const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
       if (live) p.lse2[row] = nan_row ? __int_as_float(0x7fffffff) : m_run + __log2f(l_run);
     }
