@@ -157,16 +157,15 @@ __device__ __forceinline__ void tmem_load64(uint32_t taddr, float2 (&v)[32]) {
   }
 }
 
-// A warp's 32 rows, one per lane, to global memory, 32 columns at a time.  Head
-// dims above 64 go through 2 KB of shared memory: with one row per lane a store
-// instruction touches 32 rows (and takes as many passes), through shared memory it
-// writes 64 bytes of each of eight.  With 64 columns the rows' own stores are
-// faster: shared memory is busy with the MMAs' operands (16 documents of up to
-// 2048 tokens, 8 heads of 64: forward 92 us against 99, dK/dV epilogue 1040
-// clocks against 2230).
-template <int HD>
+// A warp's 32 rows, one per lane, to global memory, 32 columns at a time.  STAGED:
+// through 2 KB of shared memory.  With one row per lane a store instruction touches
+// 32 rows (and takes as many passes); through shared memory it writes 64 bytes of
+// each of eight, but shared memory is busy with the MMAs' operands.  Measured: the
+// dK/dV kernel gains at both head dims (16 documents of up to 2048 tokens, 8 heads
+// of 64: 144 -> 138 us; 16 x 2048 tokens, 16 heads of 128: 648 -> 623), the forward
+// at 128 (377 -> 362), where 64 loses (92 -> 98).
+template <bool STAGED>
 struct WarpRows {
-  static constexpr bool STAGED = HD > 64;
   static constexpr uint32_t BYTES = STAGED ? 2048 : 0;
   uint32_t buf;
   int lane, row0;
@@ -181,13 +180,12 @@ struct WarpRows {
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = T::pack(v[e].x * scale, v[e].y * scale);
-    if (!STAGED) {
+    if constexpr (!STAGED) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (live[0] && col + 8 * u < n)
           st_global_v4(out + off[0] + col + 8 * u, w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-      return;
-    }
+    } else {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       sts128(buf + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
@@ -201,6 +199,7 @@ struct WarpRows {
       if (live[i] && col + 8 * unit < n) st_global_v4(out + off[i] + col + 8 * unit, x[0], x[1], x[2], x[3]);
     }
     __syncwarp();
+    }
   }
 };
 

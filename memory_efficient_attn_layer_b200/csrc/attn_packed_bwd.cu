@@ -97,7 +97,7 @@ struct PackedDqCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<HD>::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<true>::BYTES;
 };
 
 struct DqItem {
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     const int tok = r / p.d.p, hr = r - tok * p.d.p;
-    WarpRows<HD> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<HD>::BYTES, lane, quarter * 32);
+    WarpRows<true> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<true>::BYTES, lane, quarter * 32);
     int out_tok[4];
 #pragma unroll
     for (int i = 0; i < out.rows(); ++i) {
@@ -464,7 +464,7 @@ struct PackedDkvCfg {
   static_assert(DK_COL + HD <= 512, "TMEM budget");
   static constexpr uint32_t OFF_Q = KVB * 2 * TB, OFF_ROW = OFF_Q + ST * 2 * TB, OFF_BAR = OFF_ROW + ST * 1024;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<HD>::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<true>::BYTES;
 };
 
 struct DkvItem {
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    WarpRows<HD> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<HD>::BYTES, lane, quarter * 32);
+    WarpRows<true> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<true>::BYTES, lane, quarter * 32);
 #pragma unroll
     for (int i = 0; i < out.rows(); ++i) out.off[i] = out.row(i) * p.d.Hkv * p.d.N;
     bool ok = true;

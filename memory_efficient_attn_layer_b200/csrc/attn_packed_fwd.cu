@@ -51,7 +51,7 @@ struct PackedFwdCfg {
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<HD>::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<(HD > 64)>::BYTES;
   static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 };
 
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
     const uint32_t st = lane_base + Cfg::S_COL + 128 * x, pt = lane_base + Cfg::P_COL + Cfg::P_STEP * x;
     const uint32_t ot = lane_base + Cfg::O_COL + HD * x;
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    WarpRows<HD> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<HD>::BYTES, lane, (warp & 3) * 32);
+    WarpRows<(HD > 64)> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<(HD > 64)>::BYTES, lane, (warp & 3) * 32);
     int out_tok[4];
 #pragma unroll
     for (int i = 0; i < out.rows(); ++i) {
