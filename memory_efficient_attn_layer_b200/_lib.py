@@ -76,7 +76,8 @@ SIGNATURES = {
     "mea_attention_backward_noalloc": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _LL, _P, _P]),
     "mea_packed_plan_size": (_S, [_PD]),
     "mea_packed_attention_forward": (_I, [_PD, _P, _P, _P, _P, _P, _P, _P, _S, _P, _P]),
-    "mea_packed_attention_backward": (_I, [_PD, _P, _P, _P, _P, _P, _LL, _LL, _P, _P, _S, _P, _P, _P, _P, _P, _P]),
+    "mea_packed_backward_workspace_size": (_S, [_PD]),
+    "mea_packed_attention_backward": (_I, [_PD, _P, _P, _P, _P, _P, _LL, _LL, _P, _P, _S, _P, _S, _P, _P, _P, _P, _P]),
     "mea_layernorm_forward": (_I, [_LL, _I, _F, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
     "mea_layernorm_workspace_size": (_S, [_LL, _I]),
     "mea_layernorm_backward": (_I, [_LL, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),

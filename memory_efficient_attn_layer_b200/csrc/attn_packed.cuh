@@ -30,6 +30,8 @@ struct PackedHeader {
   int n[3];        // entries of each list
   int first, end;  // rows [first, end) belong to sequences
   int next[3];     // next tile to be drawn from each list
+  int splits;      // parts that a key tile's walk is cut into
+  int pad[3];
 };
 
 struct PackedDims {
@@ -40,6 +42,7 @@ struct PackedDims {
   int rows[3];      // tokens of a tile of each list
   int heads[3];     // tiles per entry: head groups, or key/value heads
   int cap[3];       // entries there can be
+  int most_splits;  // parts that a key tile's walk may be cut into
 };
 
 enum PackedList { LIST_Q = 0, LIST_K = 1, LIST_FWD = 2 };

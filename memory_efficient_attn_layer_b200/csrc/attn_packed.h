@@ -11,6 +11,8 @@ struct PackedPlan;
 // Checks the sizes of *d and derives the tile shape and the plan's capacity.
 int packed_dims(const mea_packed_dims* d, PackedDims* out);
 size_t packed_plan_bytes(const PackedDims& d);
+size_t packed_delta_bytes(const PackedDims& d);
+size_t packed_backward_bytes(const PackedDims& d);
 PackedPlan packed_plan_view(const PackedDims& d, void* plan);
 int run_packed_plan(const PackedDims& d, const int* cu, void* plan, int* status, cudaStream_t st);
 // Pointer, alignment and stride checks of one [total, heads, N] tensor.

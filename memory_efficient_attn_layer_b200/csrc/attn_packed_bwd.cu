@@ -18,6 +18,10 @@
 // them, are the A operands of dV and dK.  P and dS never pass through shared
 // memory, whose bandwidth the S and dP products (both operands there) need.
 //
+// With few key tiles (few key/value heads, not many rows) a tile's walk over the
+// queries is cut into parts that leave fp32 partial sums, added in their order by
+// packed_dkv_sum_kernel.
+//
 // Warps (384 threads, persistent, one CTA per SM): 0 TMA, 1 MMA issue, 2 (dK/dV)
 // lse2 and delta rows, 4..11 softmax: two warps per TMEM lane quarter, half a row
 // each.
@@ -37,6 +41,7 @@ struct PackedBwdParams {
   uint16_t* dq;        // [total, Hq, N]
   uint16_t* dk;        // [total, Hkv, N]
   uint16_t* dv;
+  float* parts;        // [splits][dK, dV][total, Hkv, N] of cut walks
   int* status;
 };
 struct PackedBwdMaps {
@@ -467,25 +472,59 @@ struct PackedDkvCfg {
   static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<true>::BYTES;
 };
 
+// Part `part` of `splits` of a key tile's walk: steps [lo, hi) over the group's
+// query tiles, `span` of them for each of `groups` sets of p heads.  A walk of
+// fewer steps has fewer parts.
 struct DkvItem {
-  int seq0, len, k0, kvh, qt0, nqt, groups, h0;
+  int seq0, len, k0, kvh, qt0, span, groups, h0, part, lo, hi;
   __device__ DkvItem() {}
-  __device__ DkvItem(const PackedDims& d, const PackedPlan& plan, int idx) {
-    const PackedTile<false> it(plan.list[LIST_K], idx, d.Hkv, 128);
+  __device__ DkvItem(const PackedDims& d, const PackedPlan& plan, int idx, int splits) {
+    part = 0;
+    if (splits > 1) {
+      const int i = idx / splits;
+      part = idx - i * splits;
+      idx = i;
+    }
+    const PackedTile<false> it(plan.list[LIST_K], idx, d.Hkv, 128);  // the first tile takes longest
     kvh = it.head;
     seq0 = it.seq0;
     len = it.len;
     k0 = it.tile * 128;
     qt0 = k0 / d.tt;
-    nqt = (len + d.tt - 1) / d.tt;
+    span = (len + d.tt - 1) / d.tt - qt0;
     const int G = d.Hq / d.Hkv;
     groups = G / d.p;
     h0 = kvh * G;
+    lo = 0;
+    hi = groups * span;
+    if (splits > 1) {
+      const int all = hi, n = parts(splits);
+      lo = part < n ? int((long long)all * part / n) : 0;
+      hi = part < n ? int((long long)all * (part + 1) / n) : 0;
+    }
   }
-  __device__ int steps() const { return groups * (nqt - qt0); }
+  __device__ int parts(int splits) const { return min(splits, groups * span); }
+  __device__ int steps() const { return hi - lo; }
+};
+// The query tile and head set of each step in turn.
+struct DkvStep {
+  int qt, gi;
+  __device__ explicit DkvStep(const DkvItem& w) : qt(w.qt0), gi(0) {
+    if (w.lo) {
+      gi = w.lo / w.span;
+      qt += w.lo - gi * w.span;
+    }
+  }
+  __device__ void next(const DkvItem& w) {
+    if (++qt == w.qt0 + w.span) {
+      qt = w.qt0;
+      ++gi;
+    }
+  }
 };
 
-template <int HD, class T>
+// CUT: walks may come in parts (the parts' bookkeeping costs the whole walks some 8%).
+template <int HD, class T, bool CUT>
 __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constant__ PackedBwdMaps maps,
                                                             const __grid_constant__ PackedBwdParams p) {
   using Cfg = PackedDkvCfg<HD>;
@@ -558,7 +597,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
-  const int n_items = p.plan.head->n[LIST_K] * p.d.Hkv;
+  const int splits = CUT ? p.plan.head->splits : 1;
+  const int n_items = p.plan.head->n[LIST_K] * p.d.Hkv * splits;
   Guard g(p.status, KID_PACKED_DKV);
 
   auto finish = [&]() {  // TMEM is freed once every warp is done with it
@@ -578,15 +618,17 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     int kvpar[2] = {-1, -1}, qpar[ST];
     for (int s = 0; s < ST; ++s) qpar[s] = -1;
     int n = 0, item = 0, raw = 0;
-    int idx = blockIdx.x;  // the grid holds no more CTAs than there can be tiles
+    int idx = blockIdx.x;
     while (g.ok) {
       int after = 0;
-      if (lead) {
-        feed.put(item, idx < n_items ? idx : -1, g);
-        if (idx < n_items) after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
+      if (lead && idx < n_items) after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
+      if (CUT && idx < n_items && !DkvItem(p.d, p.plan, idx, splits).steps()) {  // a part that a short walk does not have
+        idx = __shfl_sync(0xffffffffu, after, 0);
+        continue;
       }
+      if (lead) feed.put(item, idx < n_items ? idx : -1, g);
       if (idx >= n_items) break;
-      const DkvItem w(p.d, p.plan, idx);
+      const DkvItem w(p.d, p.plan, idx, splits);
       const int kb = item % KVB;
       if (lead && (item < KVB || mbar_wait(kv_empty(kb), uint32_t((item / KVB - 1) & 1), g, 1))) {
         mbar_expect_tx(kv_full(kb), 2 * TB);
@@ -598,11 +640,11 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
         kvpar[kb] = (item / KVB) & 1;
       }
       ++item;
-      for (int gi = 0; gi < w.groups && g.ok; ++gi)
-        for (int qt = w.qt0; qt < w.nqt; ++qt, ++n) {
+      DkvStep at(w);
+      for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
           const int s = n % ST;
           const uint32_t ph = (n / ST) & 1;
-          const int t0 = qt * p.d.tt;
+          const int t0 = at.qt * p.d.tt;
           // Rows past the sequence's end: P and dS are zero there, but the dV and
           // dK products would still multiply them by whatever the rows hold.
           const int valid = min(w.len - t0, p.d.tt) * p.d.p;
@@ -612,8 +654,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             mbar_expect_tx(full, 2 * box);
 #pragma unroll
             for (int c = 0; c < Tile::NCHUNK; ++c) {
-              tma_load_3d(sQ(s) + c * 16384, &maps.q, full, c * 64, w.h0 + gi * p.d.p, w.seq0 + t0);
-              tma_load_3d(sdO(s) + c * 16384, &maps.dO, full, c * 64, w.h0 + gi * p.d.p, w.seq0 + t0);
+              tma_load_3d(sQ(s) + c * 16384, &maps.q, full, c * 64, w.h0 + at.gi * p.d.p, w.seq0 + t0);
+              tma_load_3d(sdO(s) + c * 16384, &maps.dO, full, c * 64, w.h0 + at.gi * p.d.p, w.seq0 + t0);
             }
             qpar[s] = int(ph);
           }
@@ -657,7 +699,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       auto steps_of = [&](int item) -> int {
         while (got <= item) {
           const int idx = feed.get(got, g);
-          const int st = idx < 0 ? 0 : DkvItem(p.d, p.plan, idx).steps();
+          const int st = idx < 0 ? 0 : DkvItem(p.d, p.plan, idx, splits).steps();
           if (got % 3 == 0) item_steps[0] = st;
           if (got % 3 == 1) item_steps[1] = st;
           if (got % 3 == 2) item_steps[2] = st;
@@ -741,18 +783,18 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     for (int item = 0; g.ok; ++item) {
       const int idx = feed.get_warp(item, g, lane);
       if (!g.ok || idx < 0) break;
-      const DkvItem w(p.d, p.plan, idx);
-      for (int gi = 0; gi < w.groups && g.ok; ++gi)
-        for (int qt = w.qt0; qt < w.nqt; ++qt, ++n) {
+      const DkvItem w(p.d, p.plan, idx, splits);
+      DkvStep at(w);
+      for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
           const int s = n % ST;
           g.ok = __all_sync(0xffffffffu, mbar_wait(qdo_empty(s), ((n / ST) & 1) ^ 1, g, 11));
           if (!g.ok) break;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = lane + 32 * i;
-            const int tok = r / p.d.p, t = qt * p.d.tt + tok;
+            const int tok = r / p.d.p, t = at.qt * p.d.tt + tok;
             const bool live = tok < p.d.tt && t < w.len;
-            const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + gi * p.d.p + (r - tok * p.d.p);
+            const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + at.gi * p.d.p + (r - tok * p.d.p);
             rows[s * 256 + r] = live ? -__ldg(p.lse2 + row) : -INFINITY;  // P = 0 in rows that are not there
             rows[s * 256 + 128 + r] = live ? __ldg(p.delta + row) : 0.f;
           }
@@ -779,14 +821,14 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       const int idx = feed.get_warp(item, g, lane);
       ok = g.ok;
       if (!ok || idx < 0) break;
-      const DkvItem w(p.d, p.plan, idx);
+      const DkvItem w(p.d, p.plan, idx, splits);
       const int key = w.k0 + r;
-      for (int gi = 0; gi < w.groups && ok; ++gi)
-        for (int qt = w.qt0; qt < w.nqt; ++qt, ++n) {
+      DkvStep at(w);
+      for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
           const int s = n % ST;
           ok = __all_sync(0xffffffffu, mbar_wait(row_full(s), (n / ST) & 1, g, 12));
           if (!ok) break;
-          const int t0 = qt * p.d.tt;
+          const int t0 = at.qt * p.d.tt;
           const bool mask = t0 < w.k0 + 127;
           const int cmin = p.d.p * (key - t0) - 64 * hh;  // first of this thread's columns that sees the key
           const uint32_t sa = lane_base + Cfg::S_COL + 128 * (n % SB) + 64 * hh;
@@ -860,9 +902,9 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       if (!ok) break;
       tc_fence_after();
       // Warps 4..7 write dV, 8..11 dK.
-      uint16_t* tile = (hh ? p.dk : p.dv) + ((long long)(w.seq0 + w.k0) * p.d.Hkv + w.kvh) * p.d.N;
       const uint32_t acc = lane_base + (hh ? Cfg::DK_COL : Cfg::DV_COL);
       const float sc = hh ? p.scale : 1.0f;
+      const long long first = ((long long)(w.seq0 + w.k0) * p.d.Hkv + w.kvh) * p.d.N;  // of the tile's first row
 #pragma unroll
       for (int i = 0; i < out.rows(); ++i) out.live[i] = w.k0 + out.row(i) < w.len;
 #pragma unroll
@@ -873,9 +915,19 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           tc_fence_before();
           mbar_arrive(acc_empty);
         }
-        out.template store32<T>(v, sc, tile, c, p.d.N);
-        out.template store32<T>(v + 16, sc, tile, c + 32, p.d.N);
+        if (!CUT || splits == 1) {
+          uint16_t* tile = (hh ? p.dk : p.dv) + first;
+          out.template store32<T>(v, sc, tile, c, p.d.N);
+          out.template store32<T>(v + 16, sc, tile, c + 32, p.d.N);
+        } else if (key < w.len) {
+          float* row = p.parts + (2LL * w.part + (hh ? 0 : 1)) * p.d.total * p.d.Hkv * p.d.N + first + (long long)r * p.d.Hkv * p.d.N;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            if (c + 2 * e < p.d.N)
+              *reinterpret_cast<float4*>(row + c + 2 * e) = make_float4(v[e].x * sc, v[e].y * sc, v[e + 1].x * sc, v[e + 1].y * sc);
+        }
       }
+      __syncwarp();
       ++item;
     }
     if (!ok) g.ok = false;
@@ -883,32 +935,72 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   }
 }
 
+// dK and dV of cut walks: each key tile's parts added in their order and rounded
+// once.  A block takes 16 rows of a (tile, key/value head) at a time; nothing to
+// do where walks were not cut.
+constexpr int SUM_ROWS = 16;
+template <class T>
+__global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const __grid_constant__ PackedBwdParams p) {
+  pdl_wait();
+  const int splits = p.plan.head->splits;
+  if (splits == 1) return;
+  constexpr int CHUNKS = 128 / SUM_ROWS;
+  const int n_items = p.plan.head->n[LIST_K] * p.d.Hkv * CHUNKS, vecs = p.d.N / 4;
+  const long long set = (long long)p.d.total * p.d.Hkv * p.d.N;
+  for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
+    const DkvItem w(p.d, p.plan, idx / CHUNKS * splits, splits);
+    const int row0 = w.k0 + idx % CHUNKS * SUM_ROWS, rows = min(SUM_ROWS, w.len - row0), parts = w.parts(splits);
+    if (rows <= 0) continue;
+    const long long first = ((long long)(w.seq0 + row0) * p.d.Hkv + w.kvh) * p.d.N;
+    for (int i = threadIdx.x; i < 2 * rows * vecs; i += blockDim.x) {
+      const int which = i >= rows * vecs, k = i - which * rows * vecs;
+      const long long at = first + (long long)(k / vecs) * p.d.Hkv * p.d.N + 4 * (k % vecs);
+      const float4* f = reinterpret_cast<const float4*>(p.parts + which * set + at);
+      float4 a = __ldcs(f);
+#pragma unroll 4
+      for (int s = 1; s < parts; ++s) {
+        const float4 g = __ldcs(f + s * (set / 2));  // (2 sets of `set` floats a part)
+        a.x += g.x;
+        a.y += g.y;
+        a.z += g.z;
+        a.w += g.w;
+      }
+      *reinterpret_cast<uint2*>((which ? p.dv : p.dk) + at) = make_uint2(T::pack(a.x, a.y), T::pack(a.z, a.w));
+    }
+  }
+}
+
 template <int HD, class T>
 static int launch_packed_bwd(const PackedBwdMaps& maps, const PackedBwdParams& p, cudaStream_t st) {
   static_assert(PackedDqCfg<HD>::SMEM <= 232448 && PackedDkvCfg<HD>::SMEM <= 232448, "shared memory");
   auto dq = packed_dq_kernel<HD, T>;
-  auto dkv = packed_dkv_kernel<HD, T>;
+  auto dkv = p.d.most_splits > 1 ? packed_dkv_kernel<HD, T, true> : packed_dkv_kernel<HD, T, false>;
   if (!smem_attr_set(reinterpret_cast<const void*>(dq), int(PackedDqCfg<HD>::SMEM)) ||
       !smem_attr_set(reinterpret_cast<const void*>(dkv), int(PackedDkvCfg<HD>::SMEM)))
     return set_error(MEA_ERR_CUDA, "cudaFuncSetAttribute(packed backward) failed");
   const int sms = num_sms();
   cudaLaunchAttribute attr;
-  const long long nq = (long long)p.d.cap[LIST_Q] * p.d.hg, nk = (long long)p.d.cap[LIST_K] * p.d.Hkv;
+  const long long nq = (long long)p.d.cap[LIST_Q] * p.d.hg, nk = (long long)p.d.cap[LIST_K] * p.d.Hkv * p.d.most_splits;
   cudaLaunchConfig_t cfg = packed_launch(int(nq < sms ? nq : sms), 384, PackedDqCfg<HD>::SMEM, st, &attr);
   cudaLaunchKernelEx(&cfg, dq, maps, p);
   int rc = check_launch("packed_dq_kernel");
   if (rc != MEA_OK) return rc;
   cfg = packed_launch(int(nk < sms ? nk : sms), 384, PackedDkvCfg<HD>::SMEM, st, &attr);
   cudaLaunchKernelEx(&cfg, dkv, maps, p);
-  return check_launch("packed_dkv_kernel");
+  if ((rc = check_launch("packed_dkv_kernel")) != MEA_OK || p.d.most_splits == 1) return rc;
+  const long long blocks = (long long)p.d.cap[LIST_K] * p.d.Hkv * (128 / SUM_ROWS);
+  cfg = packed_launch(int(blocks < 8 * sms ? blocks : 8 * sms), 256, 0, st, &attr);
+  cudaLaunchKernelEx(&cfg, packed_dkv_sum_kernel<T>, p);
+  return check_launch("packed_dkv_sum_kernel");
 }
 
 }  // namespace mea
 
 extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const void* q, const void* k, const void* v,
                                              const void* o, const void* dO, long long do_row, long long do_head,
-                                             const float* lse2, void* plan, size_t plan_bytes, float* delta,
-                                             void* dq, void* dk, void* dv, int* status, void* stream) {
+                                             const float* lse2, void* plan, size_t plan_bytes, void* workspace,
+                                             size_t workspace_bytes, void* dq, void* dk, void* dv, int* status,
+                                             void* stream) {
   using namespace mea;
   PackedDims pd;
   int rc = packed_dims(d, &pd);
@@ -923,14 +1015,18 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   if ((rc = packed_check_rows("dq", dq, wq, pd.N, pd, pd.Hq)) != MEA_OK) return rc;
   if ((rc = packed_check_rows("dk", dk, wk, pd.N, pd, pd.Hkv)) != MEA_OK) return rc;
   if ((rc = packed_check_rows("dv", dv, wk, pd.N, pd, pd.Hkv)) != MEA_OK) return rc;
-  if (!lse2 || !plan || !delta)
-    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention backward: lse2, plan and delta must be non-NULL");
-  if ((reinterpret_cast<uintptr_t>(lse2) | reinterpret_cast<uintptr_t>(delta)) & 3 ||
-      reinterpret_cast<uintptr_t>(plan) & 255)
-    return set_error(MEA_ERR_ALIGNMENT, "packed attention backward: lse2 and delta must be 4-byte, plan 256-byte aligned");
+  if (!lse2 || !plan || !workspace)
+    return set_error(MEA_ERR_INVALID_ARGUMENT, "packed attention backward: lse2, plan and workspace must be non-NULL");
+  if (reinterpret_cast<uintptr_t>(lse2) & 3 || (reinterpret_cast<uintptr_t>(plan) | reinterpret_cast<uintptr_t>(workspace)) & 255)
+    return set_error(MEA_ERR_ALIGNMENT,
+                     "packed attention backward: lse2 must be 4-byte, plan and workspace 256-byte aligned");
   if (plan_bytes < packed_plan_bytes(pd))
     return set_error(MEA_ERR_WORKSPACE, "packed attention backward: plan has %zu bytes, needs %zu", plan_bytes,
                      packed_plan_bytes(pd));
+  if (workspace_bytes < packed_backward_bytes(pd))
+    return set_error(MEA_ERR_WORKSPACE, "packed attention backward: workspace has %zu bytes, needs %zu", workspace_bytes,
+                     packed_backward_bytes(pd));
+  float* delta = static_cast<float*>(workspace);
   auto st = static_cast<cudaStream_t>(stream);
   if (pd.n_seqs == 0) {  // no sequence owns a row
     if (cudaMemsetAsync(dq, 0, size_t(pd.total) * wq * 2, st) != cudaSuccess ||
@@ -952,6 +1048,7 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.lse2 = lse2;
   p.delta = delta;
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + packed_delta_bytes(pd));
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);

@@ -16,6 +16,8 @@
 // the first key rows alone walks 385 steps of 576 that an SM has).
 // The plan belongs to the call, never to a later one: a captured call builds it
 // again from the values cu_seqlens has at the replay.
+#include <algorithm>
+
 #include "attn_packed.h"
 #include "attn_packed.cuh"
 
@@ -109,6 +111,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   if (!__syncthreads_and(good)) {
     if (tid == 0) {
       p.plan.head->n[kind] = p.plan.head->next[kind] = 0;
+      if (keys) p.plan.head->splits = 1;
       if (kind == 0) {
         record_error(p.status, KID_PACKED_PLAN, 1);
         p.plan.head->first = p.plan.head->end = 0;
@@ -129,6 +132,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
     }
   }
   const int most = keys ? (longest + tt - 1) / tt : (longest + 127) >> 7;  // steps of the longest tile
+  // A part of a key tile's walk should still be some eight steps.
+  if (keys && tid == 0)
+    p.plan.head->splits = max(1, min(p.d.most_splits, most * (p.d.Hq / p.d.Hkv / p.d.p) / 8));
   const bool by_seq = p.wide[kind] && n >= 8 * max(p.at_once[kind], 1);
   if (!by_seq) {
     for (int s = tid; s < n_seqs; s += PLAN_THREADS) {
@@ -244,8 +250,19 @@ int packed_dims(const mea_packed_dims* d, PackedDims* out) {
     o.heads[i] = heads[i];
     o.cap[i] = int(cap);
   }
+  // Few key tiles (few key/value heads, not many rows): each tile's walk over the
+  // queries may be cut into parts, as many as make four for every SM.
+  const long long k_tiles = std::max<long long>(1, (long long)d->total / 128 * d->Hkv);
+  o.most_splits = int(std::min<long long>(16, std::max<long long>(1, 4LL * num_sms() / k_tiles)));
   *out = o;
   return MEA_OK;
+}
+
+// Workspace of the backward: delta [total, Hq], then the parts' dK and dV in fp32.
+size_t packed_delta_bytes(const PackedDims& d) { return up256(sizeof(float) * size_t(d.total) * d.Hq); }
+size_t packed_backward_bytes(const PackedDims& d) {
+  const size_t parts = d.most_splits > 1 ? size_t(d.most_splits) * 2 * sizeof(float) * d.total * d.Hkv * d.N : 0;
+  return packed_delta_bytes(d) + up256(parts);
 }
 
 static size_t plan_scratch(const PackedDims& d) {  // offset of the plan kernel's own space
@@ -324,6 +341,11 @@ cudaLaunchConfig_t packed_launch(int grid, int threads, size_t smem, cudaStream_
 
 }  // namespace mea
 
+extern "C" size_t mea_packed_backward_workspace_size(const mea_packed_dims* d) {
+  mea::PackedDims pd;
+  if (mea::packed_dims(d, &pd) != MEA_OK) return 0;
+  return mea::packed_backward_bytes(pd);
+}
 extern "C" size_t mea_packed_plan_size(const mea_packed_dims* d) {
   mea::PackedDims pd;
   if (mea::packed_dims(d, &pd) != MEA_OK) return 0;

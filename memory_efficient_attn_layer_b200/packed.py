@@ -79,9 +79,8 @@ def _forward(q, k, v, cu_seqlens, scale):
     L = _lib.lib()
     at = ctypes.byref(dims)
     nbytes = L.mea_packed_plan_size(at)
-    # one buffer: the plan, then lse2 [total, Hq] fp32, then the backward's delta of the same size
-    rows = 4 * total * hq
-    side = torch.empty(nbytes + 2 * rows, dtype=torch.uint8, device=q.device)
+    # one buffer: the plan, then lse2 [total, Hq] fp32
+    side = torch.empty(nbytes + 4 * total * hq, dtype=torch.uint8, device=q.device)
     p = side.data_ptr()
     _lib.launch(idx, L.mea_packed_attention_forward, at, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(),
                 o.data_ptr(), p + nbytes, p, nbytes, _lib.status_word(idx))
@@ -97,12 +96,12 @@ def _backward(ctx, grad_output):
     if side is None:
         return dq, dk, dv, None, None
     do = _rows(grad_output)
-    idx, p = q.get_device(), side.data_ptr()
-    rows = 4 * q.shape[0] * q.shape[1]
-    nbytes = side.numel() - 2 * rows
-    _lib.launch(idx, _lib.lib().mea_packed_attention_backward, ctypes.byref(ctx.dims), q.data_ptr(), k.data_ptr(),
-                v.data_ptr(), o.data_ptr(), do.data_ptr(), *do.stride()[:2], p + nbytes, p, nbytes, p + nbytes + rows,
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.status_word(idx))
+    idx, p, L, at = q.get_device(), side.data_ptr(), _lib.lib(), ctypes.byref(ctx.dims)
+    nbytes = side.numel() - 4 * q.shape[0] * q.shape[1]
+    ws = torch.empty(L.mea_packed_backward_workspace_size(at), dtype=torch.uint8, device=q.device)
+    _lib.launch(idx, L.mea_packed_attention_backward, at, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                do.data_ptr(), *do.stride()[:2], p + nbytes, p, nbytes, ws.data_ptr(), ws.numel(), dq.data_ptr(),
+                dk.data_ptr(), dv.data_ptr(), _lib.status_word(idx))
     _lib.after_launch(idx)
     return dq, dk, dv, None, None
 

@@ -79,6 +79,14 @@ def test_long_and_ragged(n, hq, hkv):
     _check([2048, 1100, 3, 777, 1, 4500, 640], hq, hkv, n, BF, seed=5)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("lens,hq,hkv,n", [([3000], 8, 1, 128), ([1500, 1, 700, 129], 7, 1, 64), ([2000, 40, 333], 4, 2, 80),
+                                           ([900], 256, 1, 64)])
+def test_walks_cut_into_parts(lens, hq, hkv, n, dt):
+    """Few key tiles and long walks: dK and dV come in parts that are added at the end."""
+    _check(lens, hq, hkv, n, dt, seed=21, before=3, behind=50)
+
+
 def test_many_sequences():
     """More sequences and tiles than the plan's block has threads."""
     g = torch.Generator().manual_seed(3)

@@ -89,7 +89,8 @@ def test_sizes_are_refused(kw, code, text):
     assert L.mea_packed_plan_size(ctypes.byref(d)) == 0
     assert text in L.mea_last_error_string()
     assert L.mea_packed_attention_forward(ctypes.byref(d), *[None] * 7, 0, None, None) == code
-    assert L.mea_packed_attention_backward(ctypes.byref(d), *[None] * 5, 0, 0, None, None, 0, *[None] * 6) == code
+    assert L.mea_packed_attention_backward(ctypes.byref(d), *[None] * 5, 0, 0, None, None, 0, None, 0, *[None] * 5) == code
+    assert L.mea_packed_backward_workspace_size(ctypes.byref(d)) == 0
 
 
 def _fake(i):
@@ -125,19 +126,22 @@ def test_small_plan_is_refused():
     L, d = _lib.lib(), _dims()
     need = L.mea_packed_plan_size(ctypes.byref(d))
     assert L.mea_packed_attention_forward(ctypes.byref(d), *[_fake(i) for i in range(7)], need - 1, None, None) == 7
-    back = [_fake(i) for i in range(5)] + [512, 64, _fake(5), _fake(6), need - 1] + [_fake(i) for i in range(7, 11)]
-    assert L.mea_packed_attention_backward(ctypes.byref(d), *back, None, None) == 7
+    work = L.mea_packed_backward_workspace_size(ctypes.byref(d))
+    for plan, ws in ((need - 1, work), (need, work - 1)):
+        back = [_fake(i) for i in range(5)] + [512, 64, _fake(5), _fake(6), plan, _fake(7), ws] + [_fake(i) for i in range(8, 11)]
+        assert L.mea_packed_attention_backward(ctypes.byref(d), *back, None, None) == 7
 
 
 @pytest.mark.parametrize("slot,value,code,text", [
     (3, None, 1, b"o is NULL"), (4, 0x7000008, 3, b"dO must be 16-byte"), (5, 500, 3, b"strides of dO"),
-    (7, None, 1, b"lse2"), (10, None, 1, b"delta"), (11, 0x7000008, 3, b"dq must be 16-byte"),
-    (13, 0x7000008, 3, b"dv must be 16-byte"),
+    (7, None, 1, b"lse2"), (10, None, 1, b"workspace"), (10, 0x7000010, 3, b"256-byte"),
+    (12, 0x7000008, 3, b"dq must be 16-byte"), (14, 0x7000008, 3, b"dv must be 16-byte"),
 ])
 def test_backward_refuses_bad_buffers_before_device_work(slot, value, code, text):
     L, d = _lib.lib(), _dims()
     need = L.mea_packed_plan_size(ctypes.byref(d))
-    args = [_fake(i) for i in range(5)] + [512, 64, _fake(5), _fake(6), need] + [_fake(i) for i in range(7, 11)]
+    work = L.mea_packed_backward_workspace_size(ctypes.byref(d))
+    args = [_fake(i) for i in range(5)] + [512, 64, _fake(5), _fake(6), need, _fake(7), work] + [_fake(i) for i in range(8, 11)]
     args[slot] = value
     assert L.mea_packed_attention_backward(ctypes.byref(d), *args, None, None) == code
     assert text in L.mea_last_error_string()
@@ -146,7 +150,7 @@ def test_backward_refuses_bad_buffers_before_device_work(slot, value, code, text
 def test_no_rows_is_nothing_to_do():
     L, d = _lib.lib(), _dims(total=0, n_seqs=3)
     assert L.mea_packed_attention_forward(ctypes.byref(d), *[None] * 7, 0, None, None) == 0
-    assert L.mea_packed_attention_backward(ctypes.byref(d), *[None] * 5, 0, 0, None, None, 0, *[None] * 6) == 0
+    assert L.mea_packed_attention_backward(ctypes.byref(d), *[None] * 5, 0, 0, None, None, 0, None, 0, *[None] * 5) == 0
 
 
 def test_plan_holds_every_tile():
