@@ -1,6 +1,7 @@
 // Causal softmax attention backward over packed sequences with grouped heads.
 //
-//   delta_i = sum_d dO_id O_id           (packed_delta_kernel)
+//   delta_i = sum_d dO_id O_id           (packed_delta_kernel; the first 128 tokens'
+//                                         again in fp32 by the dQ kernel)
 //   P_ij = exp2(scale_log2 q_i.k_j - lse2_i),  dS_ij = P_ij (dO_i.v_j - delta_i)
 //   dQ_i = scale sum_j dS_ij k_j         (packed_dq_kernel: a query tile walks its key tiles)
 //   dV_j = sum_i P_ij dO_i, dK_j = scale sum_i dS_ij q_i
@@ -37,7 +38,7 @@ struct PackedBwdParams {
   PackedPlan plan;
   float scale, scale_log2;
   const float* lse2;   // [total, Hq]
-  const float* delta;  // [total, Hq]
+  float* delta;        // [total, Hq]
   uint16_t* dq;        // [total, Hq, N]
   uint16_t* dk;        // [total, Hkv, N]
   uint16_t* dv;
@@ -101,8 +102,8 @@ struct PackedDqCfg {
   static constexpr uint32_t S_COL = 0, DP_COL = 128, DS_COL = 256, DQ_COL = 384;  // two dS buffers
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
-  static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
-  static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<true>::BYTES;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 512, OFF_X = OFF_OUT + 8 * WarpRows<true>::BYTES;
+  static constexpr size_t SMEM = 1024 + OFF_X + 1024;
 };
 
 struct DqItem {
@@ -371,8 +372,9 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
       const bool live = r < p.d.p * p.d.tt && t < w.t1;
       const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
       const float lse = live ? __ldg(p.lse2 + row) : INFINITY;  // P = 0 in rows that are not there
-      const float dl = live ? __ldg(p.delta + row) : 0.f;
-      const float2 neg_lse = make_float2(-lse, -lse), dl2 = make_float2(dl, dl);
+      const float dl = live ? p.delta[row] : 0.f;
+      const float2 neg_lse = make_float2(-lse, -lse);
+      float2 dl2 = make_float2(dl, dl);
       for (int j = 0; j < w.nkv; ++j, ++n) {
         ok = __all_sync(0xffffffffu, mbar_wait(s_full, n & 1, g, 15));
         if (!ok) break;
@@ -396,6 +398,24 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           ok = __all_sync(0xffffffffu, mbar_wait(ds_free(n & 1), ((n >> 1) - 1) & 1, g, 17));
           if (!ok) break;
           tc_fence_after();
+        }
+        if (w.nkv == 1) {
+          // The first 128 tokens of a sequence have all their keys here, so delta =
+          // sum_j P_ij dP_ij can be had from fp32 values.  From the rounded O it is off
+          // by a rounding of O, which counts where O is not yet an average of many rows.
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            sum += 2 * e > cmax ? 0.f : P[e].x * dp[e].x;
+            sum += 2 * e + 1 > cmax ? 0.f : P[e].y * dp[e].y;
+          }
+          float* xch = reinterpret_cast<float*>(smem + Cfg::OFF_X);
+          xch[hh * 128 + r] = sum;
+          named_bar_sync(2 + quarter, 64);  // the row's other half
+          sum += xch[(hh ^ 1) * 128 + r];
+          named_bar_sync(2 + quarter, 64);  // read before the next item writes
+          dl2 = make_float2(sum, sum);
+          if (live && hh == 0) p.delta[row] = sum;  // for the dK/dV kernel
         }
         auto grad = [&](auto masked) {
 #pragma unroll
@@ -796,7 +816,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             const bool live = tok < p.d.tt && t < w.len;
             const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + at.gi * p.d.p + (r - tok * p.d.p);
             rows[s * 256 + r] = live ? -__ldg(p.lse2 + row) : -INFINITY;  // P = 0 in rows that are not there
-            rows[s * 256 + 128 + r] = live ? __ldg(p.delta + row) : 0.f;
+            rows[s * 256 + 128 + r] = live ? p.delta[row] : 0.f;
           }
           mbar_arrive(row_full(s));
         }
