@@ -99,30 +99,38 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int r0, int lane) {
 }
 
 // Tiles of a persistent CTA: warp 0 draws the next number from a counter in the
-// plan (long tiles first, so the CTAs end together) and hands it to the other
-// roles through a ring of four slots; each reader copies the number and gives the
-// slot back.  Which CTA takes a tile changes no result.
+// plan (long tiles first, so the CTAs end together), works out where the tile lies,
+// and hands that to the other roles through a ring of four slots, three steps
+// before the present tile's last loads (drawn earlier, it would wait behind a long
+// tile while other CTAs run out of work); each reader gives the slot back.  (Working it out costs
+// a read of the plan and two divisions, about 1000 clocks, on every role's path.)
+// Which CTA takes a tile changes no result.
+template <class Item>
 struct Feed {
-  static constexpr int SLOTS = 4;
+  static constexpr int SLOTS = 4, WORDS = sizeof(Item) / 4;
+  static constexpr uint32_t BYTES = SLOTS * sizeof(Item);
   uint32_t full, empty;  // mbarriers, SLOTS each
-  volatile int* idx;
-  __device__ void put(int n, int value, Guard& g) const {  // one thread
+  Item* slot;
+  __device__ void put(int n, const Item& w, Guard& g) const {  // one thread
     if (!mbar_wait(empty + 8u * (n % SLOTS), ((n / SLOTS) & 1) ^ 1, g, 30)) return;
-    idx[n % SLOTS] = value;
+    slot[n % SLOTS] = w;
     mbar_arrive(full + 8u * (n % SLOTS));
   }
-  __device__ int get(int n, Guard& g) const {  // one thread; -1: no more tiles
-    if (!mbar_wait(full + 8u * (n % SLOTS), (n / SLOTS) & 1, g, 31)) return -1;
-    const int v = idx[n % SLOTS];
+  __device__ bool get(int n, Item& w, Guard& g) const {  // one thread; false: no more tiles
+    if (!mbar_wait(full + 8u * (n % SLOTS), (n / SLOTS) & 1, g, 31)) return false;
+    w = slot[n % SLOTS];
     mbar_arrive(empty + 8u * (n % SLOTS));
-    return v;
+    return w.there();
   }
-  __device__ int get_warp(int n, Guard& g, int lane) const {  // a whole warp
-    int v = -1;
-    if (lane == 0) v = get(n, g);
-    v = __shfl_sync(0xffffffffu, v, 0);
-    g.ok = __shfl_sync(0xffffffffu, int(g.ok), 0) && g.ok;
-    return v;
+  // A whole warp: the tile stays in its slot (where its fields cost no registers)
+  // until done().
+  __device__ const volatile Item* look(int n, Guard& g) const {
+    g.ok = __all_sync(0xffffffffu, mbar_wait(full + 8u * (n % SLOTS), (n / SLOTS) & 1, g, 31));
+    return slot + n % SLOTS;
+  }
+  __device__ void done(int n, int lane) const {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8u * (n % SLOTS));
   }
 };
 

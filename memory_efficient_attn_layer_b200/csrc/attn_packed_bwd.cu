@@ -102,14 +102,17 @@ struct PackedDqCfg {
   static constexpr uint32_t S_COL = 0, DP_COL = 128, DS_COL = 256, DQ_COL = 384;  // two dS buffers
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
-  static constexpr uint32_t OFF_OUT = OFF_BAR + 512, OFF_X = OFF_OUT + 8 * WarpRows<true>::BYTES;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 768, OFF_X = OFF_OUT + 8 * WarpRows<true>::BYTES;
   static constexpr size_t SMEM = 1024 + OFF_X + 1024;
 };
 
 struct DqItem {
-  int seq0, len, t0, t1, nkv, h0, kvh;
+  int seq0, len, t0, t1, h0, kvh;
+  int nkv;  // key tiles; 0: no item
   __device__ DqItem() {}
-  __device__ DqItem(const PackedDims& d, const PackedPlan& plan, int idx) {
+  __device__ DqItem(const PackedDims& d, const PackedPlan& plan, int idx, int n_items) {
+    nkv = 0;
+    if (idx >= n_items) return;
     const PackedTile<true> it(plan.list[LIST_Q], idx, d.hg, d.tt);
     seq0 = it.seq0;
     len = it.len;
@@ -119,6 +122,7 @@ struct DqItem {
     h0 = it.head * d.p;
     kvh = h0 / (d.Hq / d.Hkv);
   }
+  __device__ bool there() const volatile { return nkv > 0; }
 };
 
 template <int HD, class T>
@@ -152,8 +156,8 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
   auto ds_free = [&](int b) { return b0 + 8u * (17 + b); };        // read by the dQ MMAs, per buffer
   const uint32_t dq_full = b0 + 8u * 19, dq_empty = b0 + 8u * 20;  // an item's dQ complete / read out
   const uint32_t k_raw = b0 + 8u * 21, drain_bar = b0 + 8u * 22;
-  const Feed feed{b0 + 8u * 23, b0 + 8u * 27, reinterpret_cast<int*>(bars + 31)};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
+  const Feed<DqItem> feed{b0 + 8u * 23, b0 + 8u * 27, reinterpret_cast<DqItem*>(bars + 32)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -170,7 +174,8 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     mbar_init(dq_empty, 256);
     mbar_init(k_raw, 1);
     mbar_init(drain_bar, 1);
-    for (int i = 0; i < Feed::SLOTS; ++i) {
+    static_assert(8 * 32 + Feed<DqItem>::BYTES <= 768, "barrier space");
+    for (int i = 0; i < feed.SLOTS; ++i) {
       mbar_init(feed.full + 8u * i, 1);
       mbar_init(feed.empty + 8u * i, 9);  // MMA, eight softmax warps
     }
@@ -196,15 +201,9 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     for (int s = 0; s < KS; ++s) kpar[s] = -1;
     for (int s = 0; s < VS; ++s) vpar[s] = -1;
     int n = 0, item = 0, raw = 0;
-    int idx = blockIdx.x;  // the grid holds no more CTAs than there can be tiles
-    while (g.ok) {
-      int after = 0;
-      if (lead) {
-        feed.put(item, idx < n_items ? idx : -1, g);
-        if (idx < n_items) after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_Q], 1);
-      }
-      if (idx >= n_items) break;
-      const DqItem w(p.d, p.plan, idx);
+    DqItem w(p.d, p.plan, blockIdx.x, n_items), next;
+    if (lead) feed.put(0, w, g);
+    while (w.there() && g.ok) {
       const int qb = item % QB;
       if (lead && (item < QB || mbar_wait(q_empty(qb), uint32_t((item / QB - 1) & 1), g, 1))) {
         mbar_expect_tx(q_full(qb), 2u * uint32_t(p.d.p * p.d.tt) * 128 * Tile::NCHUNK);
@@ -239,6 +238,12 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
             vpar[sv] = int(pv);
           }
         }
+        if (j == max(w.nkv - 3, 0)) {
+          int idx = 0;
+          if (lead) idx = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_Q], 1);
+          next = DqItem(p.d, p.plan, __shfl_sync(0xffffffffu, idx, 0), n_items);
+          if (lead) feed.put(item, next, g);  // (item counts this one already)
+        }
         g.ok = __all_sync(0xffffffffu, g.ok);
         if (!g.ok) break;
         if (tail) {
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           if (lead) mbar_arrive(k_full(sk));
         }
       }
-      idx = __shfl_sync(0xffffffffu, after, 0);
+      w = next;
     }
     if (lead) {
       if (!g.ok) {
@@ -279,8 +284,8 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
       // S and dP run one step ahead of dQ, across items: (n1, item1, j1) is their next step.
       int n1 = 0, item1 = 0, j1 = 0, nkv1 = 0;  // nkv1 = 0: no more items
       auto settle = [&]() {
-        const int idx = feed.get(item1, g);
-        nkv1 = idx < 0 ? 0 : DqItem(p.d, p.plan, idx).nkv;
+        DqItem w;
+        nkv1 = feed.get(item1, w, g) ? w.nkv : 0;
       };
       settle();
       auto issue_s = [&]() -> bool {
@@ -355,31 +360,25 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     const int tok = r / p.d.p, hr = r - tok * p.d.p;
     WarpRows<true> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<true>::BYTES, lane, quarter * 32);
-    int out_tok[4];
-#pragma unroll
-    for (int i = 0; i < out.rows(); ++i) {
-      out_tok[i] = out.row(i) / p.d.p;
-      out.off[i] = (out_tok[i] * p.d.Hq + out.row(i) - out_tok[i] * p.d.p) * p.d.N;
-    }
     bool ok = true;
     int n = 0, item = 0;
     while (ok) {
-      const int idx = feed.get_warp(item, g, lane);
+      const volatile DqItem& w = *feed.look(item, g);
       ok = g.ok;
-      if (!ok || idx < 0) break;
-      const DqItem w(p.d, p.plan, idx);
-      const int t = w.t0 + tok;
+      if (!ok || !w.there()) break;
+      const int nkv = w.nkv, t0 = w.t0;
+      const int t = t0 + tok;
       const bool live = r < p.d.p * p.d.tt && t < w.t1;
       const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
       const float lse = live ? __ldg(p.lse2 + row) : INFINITY;  // P = 0 in rows that are not there
       const float dl = live ? p.delta[row] : 0.f;
       const float2 neg_lse = make_float2(-lse, -lse);
       float2 dl2 = make_float2(dl, dl);
-      for (int j = 0; j < w.nkv; ++j, ++n) {
+      for (int j = 0; j < nkv; ++j, ++n) {
         ok = __all_sync(0xffffffffu, mbar_wait(s_full, n & 1, g, 15));
         if (!ok) break;
         tc_fence_after();
-        const bool mask = 128 * j + 127 > w.t0;
+        const bool mask = 128 * j + 127 > t0;
         const int cmax = t - 128 * j - 64 * hh;  // last of this thread's columns that the row sees
         float2 P[32];
         tmem_load64(lane_base + Cfg::S_COL + 64 * hh, P);
@@ -399,7 +398,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           if (!ok) break;
           tc_fence_after();
         }
-        if (w.nkv == 1) {
+        if (nkv == 1) {
           // The first 128 tokens of a sequence have all their keys here, so delta =
           // sum_j P_ij dP_ij can be had from fp32 values.  From the rounded O it is off
           // by a rounding of O, which counts where O is not yet an average of many rows.
@@ -457,10 +456,15 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
       tc_fence_before();
       mbar_arrive(dq_empty);
 #pragma unroll
-      for (int i = 0; i < out.rows(); ++i) out.live[i] = out_tok[i] < w.t1 - w.t0;
-      uint16_t* tile = p.dq + ((long long)(w.seq0 + w.t0) * p.d.Hq + w.h0) * p.d.N;
+      for (int i = 0; i < out.rows(); ++i) {
+        const int row_tok = out.row(i) / p.d.p;
+        out.off[i] = (row_tok * p.d.Hq + out.row(i) - row_tok * p.d.p) * p.d.N;
+        out.live[i] = row_tok < w.t1 - t0;
+      }
+      uint16_t* tile = p.dq + ((long long)(w.seq0 + t0) * p.d.Hq + w.h0) * p.d.N;
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) out.template store32<T>(dq + 16 * c, p.scale, tile, hh * (HD / 2) + 32 * c, p.d.N);
+      feed.done(item, lane);
       ++item;
     }
     // The last two steps' ds_free have landed before this CTA's shared memory goes away.
@@ -488,7 +492,7 @@ struct PackedDkvCfg {
   static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
   static_assert(DK_COL + HD <= 512, "TMEM budget");
   static constexpr uint32_t OFF_Q = KVB * 2 * TB, OFF_ROW = OFF_Q + ST * 2 * TB, OFF_BAR = OFF_ROW + ST * 1024;
-  static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 768;
   static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<true>::BYTES;
 };
 
@@ -496,9 +500,12 @@ struct PackedDkvCfg {
 // query tiles, `span` of them for each of `groups` sets of p heads.  A walk of
 // fewer steps has fewer parts.
 struct DkvItem {
-  int seq0, len, k0, kvh, qt0, span, groups, h0, part, lo, hi;
+  int seq0, len, k0, kvh, qt0, span, h0, part;
+  int lo, hi;  // lo = hi: a part that a short walk does not have; lo < 0: no item
   __device__ DkvItem() {}
-  __device__ DkvItem(const PackedDims& d, const PackedPlan& plan, int idx, int splits) {
+  __device__ DkvItem(const PackedDims& d, const PackedPlan& plan, int idx, int splits, int n_items) {
+    lo = hi = -1;
+    if (idx >= n_items) return;
     part = 0;
     if (splits > 1) {
       const int i = idx / splits;
@@ -512,19 +519,18 @@ struct DkvItem {
     k0 = it.tile * 128;
     qt0 = k0 / d.tt;
     span = (len + d.tt - 1) / d.tt - qt0;
-    const int G = d.Hq / d.Hkv;
-    groups = G / d.p;
-    h0 = kvh * G;
+    h0 = kvh * (d.Hq / d.Hkv);
     lo = 0;
-    hi = groups * span;
+    hi = d.Hq / d.Hkv / d.p * span;
     if (splits > 1) {
-      const int all = hi, n = parts(splits);
+      const int all = hi, n = parts(d, splits);
       lo = part < n ? int((long long)all * part / n) : 0;
       hi = part < n ? int((long long)all * (part + 1) / n) : 0;
     }
   }
-  __device__ int parts(int splits) const { return min(splits, groups * span); }
-  __device__ int steps() const { return hi - lo; }
+  __device__ int parts(const PackedDims& d, int splits) const { return min(splits, d.Hq / d.Hkv / d.p * span); }
+  __device__ int steps() const volatile { return hi - lo; }
+  __device__ bool there() const volatile { return lo >= 0; }
 };
 // The query tile and head set of each step in turn.
 struct DkvStep {
@@ -577,7 +583,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
   const uint32_t acc_full = b0 + 8u * 22, acc_empty = b0 + 8u * 23;  // an item's dK, dV complete / read out
   const uint32_t raw_bar = b0 + 8u * 24, drain_bar = b0 + 8u * 25;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
-  const Feed feed{b0 + 8u * 26, b0 + 8u * 30, reinterpret_cast<int*>(bars + 35)};
+  const Feed<DkvItem> feed{b0 + 8u * 26, b0 + 8u * 30, reinterpret_cast<DkvItem*>(bars + 36)};
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -594,7 +600,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     mbar_init(acc_empty, 256);
     mbar_init(raw_bar, 1);
     mbar_init(drain_bar, 1);
-    for (int i = 0; i < Feed::SLOTS; ++i) {
+    static_assert(8 * 36 + Feed<DkvItem>::BYTES <= 768, "barrier space");
+    for (int i = 0; i < feed.SLOTS; ++i) {
       mbar_init(feed.full + 8u * i, 1);
       mbar_init(feed.empty + 8u * i, 10);  // MMA, warp 2, eight softmax warps
     }
@@ -638,17 +645,17 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     int kvpar[2] = {-1, -1}, qpar[ST];
     for (int s = 0; s < ST; ++s) qpar[s] = -1;
     int n = 0, item = 0, raw = 0;
-    int idx = blockIdx.x;
-    while (g.ok) {
-      int after = 0;
-      if (lead && idx < n_items) after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
-      if (CUT && idx < n_items && !DkvItem(p.d, p.plan, idx, splits).steps()) {  // a part that a short walk does not have
-        idx = __shfl_sync(0xffffffffu, after, 0);
-        continue;
+    auto draw = [&](int idx) {  // tile idx, or the next one that has steps
+      DkvItem w(p.d, p.plan, idx, splits, n_items);
+      while (CUT && w.there() && !w.steps()) {
+        if (lead) idx = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
+        w = DkvItem(p.d, p.plan, __shfl_sync(0xffffffffu, idx, 0), splits, n_items);
       }
-      if (lead) feed.put(item, idx < n_items ? idx : -1, g);
-      if (idx >= n_items) break;
-      const DkvItem w(p.d, p.plan, idx, splits);
+      return w;
+    };
+    DkvItem w = draw(blockIdx.x), next;
+    if (lead) feed.put(0, w, g);
+    while (w.there() && g.ok) {
       const int kb = item % KVB;
       if (lead && (item < KVB || mbar_wait(kv_empty(kb), uint32_t((item / KVB - 1) & 1), g, 1))) {
         mbar_expect_tx(kv_full(kb), 2 * TB);
@@ -679,6 +686,12 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             }
             qpar[s] = int(ph);
           }
+          if (k == max(w.hi - 3, w.lo)) {
+            int idx = 0;
+            if (lead) idx = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
+            next = draw(__shfl_sync(0xffffffffu, idx, 0));
+            if (lead) feed.put(item, next, g);  // (item counts this one already)
+          }
           g.ok = __all_sync(0xffffffffu, g.ok);
           if (!g.ok) break;
           if (tail) {
@@ -692,7 +705,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             if (lead) mbar_arrive(qdo_full(s));
           }
         }
-      idx = __shfl_sync(0xffffffffu, after, 0);
+      w = next;
     }
     if (lead) {
       if (!g.ok) {
@@ -718,8 +731,8 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       int item_steps[3], got = 0;
       auto steps_of = [&](int item) -> int {
         while (got <= item) {
-          const int idx = feed.get(got, g);
-          const int st = idx < 0 ? 0 : DkvItem(p.d, p.plan, idx, splits).steps();
+          DkvItem w;
+          const int st = feed.get(got, w, g) ? w.steps() : 0;
           if (got % 3 == 0) item_steps[0] = st;
           if (got % 3 == 1) item_steps[1] = st;
           if (got % 3 == 2) item_steps[2] = st;
@@ -801,9 +814,10 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     // ---------------- -lse2 and delta of each step's 128 query rows ----------------
     int n = 0;
     for (int item = 0; g.ok; ++item) {
-      const int idx = feed.get_warp(item, g, lane);
-      if (!g.ok || idx < 0) break;
-      const DkvItem w(p.d, p.plan, idx, splits);
+      const volatile DkvItem& slot = *feed.look(item, g);
+      if (!g.ok || !slot.there()) break;
+      const DkvItem w = const_cast<const DkvItem&>(slot);
+      feed.done(item, lane);
       DkvStep at(w);
       for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
           const int s = n % ST;
@@ -838,18 +852,17 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     bool ok = true;
     int n = 0, item = 0;
     while (ok) {
-      const int idx = feed.get_warp(item, g, lane);
+      const volatile DkvItem& w = *feed.look(item, g);
       ok = g.ok;
-      if (!ok || idx < 0) break;
-      const DkvItem w(p.d, p.plan, idx, splits);
-      const int key = w.k0 + r;
-      DkvStep at(w);
-      for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
+      if (!ok || !w.there()) break;
+      const int k0 = w.k0, key = k0 + r, qt0 = w.qt0, qt_end = qt0 + w.span;
+      int qt = qt0 + w.lo % w.span;
+      for (int k = w.hi - w.lo; k > 0; --k, ++n, qt = qt + 1 == qt_end ? qt0 : qt + 1) {
           const int s = n % ST;
           ok = __all_sync(0xffffffffu, mbar_wait(row_full(s), (n / ST) & 1, g, 12));
           if (!ok) break;
-          const int t0 = at.qt * p.d.tt;
-          const bool mask = t0 < w.k0 + 127;
+          const int t0 = qt * p.d.tt;
+          const bool mask = t0 < k0 + 127;
           const int cmin = p.d.p * (key - t0) - 64 * hh;  // first of this thread's columns that sees the key
           const uint32_t sa = lane_base + Cfg::S_COL + 128 * (n % SB) + 64 * hh;
           const uint32_t da = lane_base + Cfg::DP_COL + 64 * hh;
@@ -924,9 +937,9 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       // Warps 4..7 write dV, 8..11 dK.
       const uint32_t acc = lane_base + (hh ? Cfg::DK_COL : Cfg::DV_COL);
       const float sc = hh ? p.scale : 1.0f;
-      const long long first = ((long long)(w.seq0 + w.k0) * p.d.Hkv + w.kvh) * p.d.N;  // of the tile's first row
+      const long long first = ((long long)(w.seq0 + k0) * p.d.Hkv + w.kvh) * p.d.N;  // of the tile's first row
 #pragma unroll
-      for (int i = 0; i < out.rows(); ++i) out.live[i] = w.k0 + out.row(i) < w.len;
+      for (int i = 0; i < out.rows(); ++i) out.live[i] = k0 + out.row(i) < w.len;
 #pragma unroll
       for (int c = 0; c < HD; c += 64) {
         float2 v[32];
@@ -947,7 +960,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
               *reinterpret_cast<float4*>(row + c + 2 * e) = make_float4(v[e].x * sc, v[e].y * sc, v[e + 1].x * sc, v[e + 1].y * sc);
         }
       }
-      __syncwarp();
+      feed.done(item, lane);
       ++item;
     }
     if (!ok) g.ok = false;
@@ -968,8 +981,8 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const __grid_consta
   const int n_items = p.plan.head->n[LIST_K] * p.d.Hkv * CHUNKS, vecs = p.d.N / 4;
   const long long set = (long long)p.d.total * p.d.Hkv * p.d.N;
   for (int idx = blockIdx.x; idx < n_items; idx += gridDim.x) {
-    const DkvItem w(p.d, p.plan, idx / CHUNKS * splits, splits);
-    const int row0 = w.k0 + idx % CHUNKS * SUM_ROWS, rows = min(SUM_ROWS, w.len - row0), parts = w.parts(splits);
+    const DkvItem w(p.d, p.plan, idx / CHUNKS * splits, splits, n_items / CHUNKS * splits);
+    const int row0 = w.k0 + idx % CHUNKS * SUM_ROWS, rows = min(SUM_ROWS, w.len - row0), parts = w.parts(p.d, splits);
     if (rows <= 0) continue;
     const long long first = ((long long)(w.seq0 + row0) * p.d.Hkv + w.kvh) * p.d.N;
     for (int i = threadIdx.x; i < 2 * rows * vecs; i += blockDim.x) {

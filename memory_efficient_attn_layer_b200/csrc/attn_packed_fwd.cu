@@ -50,7 +50,7 @@ struct PackedFwdCfg {
   static constexpr uint32_t O_COL = SEP_P ? 384 : 256;
   static constexpr uint32_t TMEM_COLS = 512;
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
-  static constexpr uint32_t OFF_OUT = OFF_BAR + 512;
+  static constexpr uint32_t OFF_OUT = OFF_BAR + 768;
   static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<(HD > 64)>::BYTES;
   static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 };
@@ -86,23 +86,25 @@ __device__ __forceinline__ bool clear_nonfinite(uint32_t tile, int r0, int r1, i
 
 // One item: the query tiles [t0, t0 + tt) and, with two streams, [t0 + tt, t0 + 2 tt) of a sequence.
 struct FwdItem {
-  int seq0, len, t0, end, h0, kvh;
+  int seq0, t0, end, h0, kvh;
   int nkv[2];  // key tiles of each stream (0: no such tile)
-  int n;       // the larger: stream 1 never has fewer, unless it is not there
+  int n;       // the larger: stream 1 never has fewer, unless it is not there; -1: no item
   __device__ FwdItem() {}
-  __device__ FwdItem(const PackedFwdParams& p, int idx) {
+  __device__ FwdItem(const PackedFwdParams& p, int idx, int n_items) {
+    n = -1;
+    if (idx >= n_items) return;
     const int rows = p.d.rows[LIST_FWD];
     const PackedTile<true> it(p.plan.list[LIST_FWD], idx, p.d.hg, rows);
     seq0 = it.seq0;
-    len = it.len;
     t0 = it.tile * rows;
-    end = min(t0 + rows, len);
+    end = min(t0 + rows, it.len);
     h0 = it.head * p.d.p;
     kvh = h0 / (p.d.Hq / p.d.Hkv);
-    nkv[0] = (min(t0 + p.d.tt, len) + 127) >> 7;
+    nkv[0] = (min(t0 + p.d.tt, end) + 127) >> 7;
     nkv[1] = end > t0 + p.d.tt ? (end + 127) >> 7 : 0;
     n = max(nkv[0], nkv[1]);
   }
+  __device__ bool there() const volatile { return n > 0; }
 };
 
 template <int HD, class T>
@@ -137,9 +139,9 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
   auto o_full = [&](int x) { return b0 + 8u * (22 + x); };   // an item's O_x complete
   auto o_empty = [&](int x) { return b0 + 8u * (24 + x); };  // and read out
   const uint32_t drain_bar = b0 + 8u * 26;
-  const Feed feed{b0 + 8u * 28, b0 + 8u * 32, reinterpret_cast<int*>(bars + 36)};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
-  volatile int* bad = reinterpret_cast<int*>(bars + 40);  // per item (mod 4) and stream: V held inf or NaN behind the mask
+  const Feed<FwdItem> feed{b0 + 8u * 28, b0 + 8u * 32, reinterpret_cast<FwdItem*>(bars + 42)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 36);
+  volatile int* bad = reinterpret_cast<int*>(bars + 37);  // per item (mod 4) and stream: V held inf or NaN behind the mask
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -153,7 +155,8 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
       mbar_init(o_empty(x), 128);
     }
     mbar_init(drain_bar, 1);
-    for (int i = 0; i < Feed::SLOTS; ++i) {
+    static_assert(8 * 42 + Feed<FwdItem>::BYTES <= 768, "barrier space");
+    for (int i = 0; i < feed.SLOTS; ++i) {
       mbar_init(feed.full + 8u * i, 1);
       mbar_init(feed.empty + 8u * i, 10);  // MMA, warp 2, eight softmax warps
     }
@@ -191,12 +194,11 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
         int qpar[2] = {-1, -1}, kpar[KS], vpar[VS];
         for (int s = 0; s < KS; ++s) kpar[s] = -1;
         for (int s = 0; s < VS; ++s) vpar[s] = -1;
-        int n = 0, idx = blockIdx.x;
-        for (int item = 0; g.ok; ++item) {
-          feed.put(item, idx < n_items ? idx : -1, g);
-          if (idx >= n_items) break;
-          const int after = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_FWD], 1);
-          const FwdItem w(p, idx);
+        int n = 0;
+        FwdItem w(p, blockIdx.x, n_items);
+        feed.put(0, w, g);
+        for (int item = 0; w.there() && g.ok; ++item) {
+          FwdItem next;
           const int qb = item % QB;
           if (item >= QB && !mbar_wait(q_empty(qb), uint32_t((item / QB - 1) & 1), g, 1)) break;
           mbar_expect_tx(q_full(qb), w.nkv[1] ? 2 * box : box);
@@ -220,8 +222,12 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
             for (int c = 0; c < Tile::NCHUNK; ++c)
               tma_load_3d(sV(sv) + c * 16384, &maps.v, v_raw(sv), c * 64, w.kvh, w.seq0 + j * 128);
             vpar[sv] = int(pv);
+            if (j == max(w.n - 3, 0)) {
+              next = FwdItem(p, int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_FWD], 1), n_items);
+              feed.put(item + 1, next, g);
+            }
           }
-          idx = after;
+          w = next;
         }
         if (!g.ok) {
           for (int b = 0; b < QB; ++b)
@@ -245,12 +251,6 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
       if (elect_one()) {
         bool any = false;
         int done[2] = {0, 0};  // steps of each stream so far (parities of p_full, s_empty)
-        auto get = [&](int item, FwdItem& w) -> bool {
-          const int idx = feed.get(item, g);
-          if (idx < 0) return false;
-          w = FwdItem(p, idx);
-          return true;
-        };
         // S_x(j) of an item whose first K tile is number k0; the last stream to use the tile gives it back.
         auto issue_s = [&](const FwdItem& w, int item, int k0, int x, int j) -> bool {
           const int qb = item % QB, sk = (k0 + j) % KS;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
         };
         FwdItem w;
         int k0 = 0, outs[2] = {0, 0};  // K tile number at the item's start; items that each stream has had
-        bool have = get(0, w);
+        bool have = feed.get(0, w, g);
         if (have && issue_s(w, 0, 0, 0, 0) && w.nkv[1]) issue_s(w, 0, 0, 1, 0);
         for (int item = 0; have && g.ok; ++item) {
           for (int j = 0; j < w.n && g.ok; ++j) {
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
           if (!g.ok) break;
           k0 += w.n;
           FwdItem nx;
-          have = get(item + 1, nx);
+          have = feed.get(item + 1, nx, g);
           if (have) {
             // SEP_P: the last scores must be in registers before the next item's are written.
             for (int x = 0; x < (nx.nkv[1] ? 2 : 1); ++x) {
@@ -321,9 +321,8 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
       // ---------------- V tiles: passed on, or looked over where the mask cuts them ----------------
       int n = 0;
       for (int item = 0; g.ok; ++item) {
-        const int idx = feed.get_warp(item, g, lane);
-        if (!g.ok || idx < 0) break;
-        const FwdItem w(p, idx);
+        const volatile FwdItem& w = *feed.look(item, g);
+        if (!g.ok || !w.there()) break;
         bool found = false;
         for (int j = 0; j < w.n; ++j, ++n) {
           const int sv = n % VS;
@@ -342,6 +341,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
           __syncwarp();
           if (lane == 0) mbar_arrive(v_full(sv));
         }
+        feed.done(item, lane);
       }
     }
     finish();
@@ -355,27 +355,22 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
                  gridDim.x, threadIdx.x - 128, 256);
     const int x = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;
-    const int tok = r / p.d.p, hr = r - tok * p.d.p;
+    const int tok = r / p.d.p;
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t st = lane_base + Cfg::S_COL + 128 * x, pt = lane_base + Cfg::P_COL + Cfg::P_STEP * x;
     const uint32_t ot = lane_base + Cfg::O_COL + HD * x;
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    WarpRows<(HD > 64)> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<(HD > 64)>::BYTES, lane, (warp & 3) * 32);
-    int out_tok[4];
-#pragma unroll
-    for (int i = 0; i < out.rows(); ++i) {
-      out_tok[i] = out.row(i) / p.d.p;
-      out.off[i] = (out_tok[i] * p.d.Hq + out.row(i) - out_tok[i] * p.d.p) * p.d.N;
-    }
     bool ok = true;
     int n = 0, outs = 0;  // steps and items of this stream
     for (int item = 0; ok; ++item) {
-      const int idx = feed.get_warp(item, g, lane);
+      const volatile FwdItem& w = *feed.look(item, g);
       ok = g.ok;
-      if (!ok || idx < 0) break;
-      const FwdItem w(p, idx);
-      const int nkv = x ? w.nkv[1] : w.nkv[0];
-      if (!nkv) continue;
+      if (!ok || !w.there()) break;
+      const int nkv = w.nkv[x];
+      if (!nkv) {
+        feed.done(item, lane);
+        continue;
+      }
       const int first = w.t0 + x * p.d.tt;  // the tile's first token
       const int t = first + tok;
       const bool live = tok < p.d.tt && t < w.end;
@@ -504,13 +499,19 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
         }
       }
       __syncwarp();
+      WarpRows<(HD > 64)> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<(HD > 64)>::BYTES, lane, (warp & 3) * 32);
 #pragma unroll
-      for (int i = 0; i < out.rows(); ++i) out.live[i] = out_tok[i] < min(p.d.tt, w.end - first);
+      for (int i = 0; i < out.rows(); ++i) {
+        const int row_tok = out.row(i) / p.d.p;
+        out.off[i] = (row_tok * p.d.Hq + out.row(i) - row_tok * p.d.p) * p.d.N;
+        out.live[i] = row_tok < min(p.d.tt, w.end - first);
+      }
       uint16_t* tile = static_cast<uint16_t*>(p.o) + ((long long)(w.seq0 + first) * p.d.Hq + w.h0) * p.d.N;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) out.template store32<T>(f + 16 * c, inv_l, tile, 32 * c, p.d.N);
-      const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + hr;
+      const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + r - tok * p.d.p;
       if (live) p.lse2[row] = nan_row ? __int_as_float(0x7fffffff) : m_run + __log2f(l_run);
+      feed.done(item, lane);
     }
     // The last pv_done has landed before this CTA's shared memory goes away.
     if (Cfg::SEP_P && ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done(x), (n - 1) & 1, g, 18));
