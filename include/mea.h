@@ -232,11 +232,11 @@ int mea_packed_attention_forward(const mea_packed_dims* d, const void* q, const 
 /* Bytes of workspace of the backward; 256-byte aligned device memory. */
 size_t mea_packed_backward_workspace_size(const mea_packed_dims* d);
 /* dq, dk, dv of the same call from its o, lse2 and plan and from dO (strides
- * as q's).  The plan's list stays, two
- * counters in it are used: backward calls that overlap need plans of their own. */
+ * as q's).  The plan is only read: backward calls of one forward may overlap,
+ * each with its own workspace. */
 int mea_packed_attention_backward(const mea_packed_dims* d, const void* q, const void* k, const void* v, const void* o,
                                   const void* dO, long long do_row, long long do_head, const float* lse2,
-                                  void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes, void* dq,
+                                  const void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes, void* dq,
                                   void* dk, void* dv, int* status, void* stream);
 
 /* ---------------------------------------------------------------- no allocation

@@ -11,6 +11,8 @@ struct PackedPlan;
 // Checks the sizes of *d and derives the tile shape and the plan's capacity.
 int packed_dims(const mea_packed_dims* d, PackedDims* out);
 size_t packed_plan_bytes(const PackedDims& d);
+// The backward's workspace: its tile counters, delta [total, Hq], then the parts' dK and dV in fp32.
+constexpr size_t PACKED_COUNTERS = 256;
 size_t packed_delta_bytes(const PackedDims& d);
 size_t packed_backward_bytes(const PackedDims& d);
 PackedPlan packed_plan_view(const PackedDims& d, void* plan);

@@ -39,6 +39,7 @@ struct PackedBwdParams {
   float scale, scale_log2;
   const float* lse2;   // [total, Hq]
   float* delta;        // [total, Hq]
+  int* next;           // next tile to be drawn from LIST_Q and LIST_K
   uint16_t* dq;        // [total, Hq, N]
   uint16_t* dk;        // [total, Hkv, N]
   uint16_t* dv;
@@ -55,11 +56,11 @@ struct PackedBwdMaps {
 // counters that the next two kernels draw their tiles from.
 constexpr int DELTA_ROWS = 64;  // rows per 256-thread block
 template <class T>
-__global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, PackedHeader* head, const uint16_t* o,
+__global__ void __launch_bounds__(256) packed_delta_kernel(PackedDims d, const PackedHeader* head, int* next, const uint16_t* o,
                                                            const uint16_t* dO, long long do_row, long long do_head,
                                                            float* delta, uint4* dq, uint4* dk, uint4* dv) {
   pdl_launch();
-  if (blockIdx.x == 0 && threadIdx.x == 0) head->next[LIST_Q] = head->next[LIST_K] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) next[LIST_Q] = next[LIST_K] = 0;
   const long long rows = (long long)d.total * d.Hq;
   const int sub = threadIdx.x & 15;
   const long long r0 = (long long)blockIdx.x * DELTA_ROWS + (threadIdx.x >> 4);
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
         }
         if (j == max(w.nkv - 3, 0)) {
           int idx = 0;
-          if (lead) idx = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_Q], 1);
+          if (lead) idx = int(gridDim.x) + atomicAdd(p.next + LIST_Q, 1);
           next = DqItem(p.d, p.plan, __shfl_sync(0xffffffffu, idx, 0), n_items);
           if (lead) feed.put(item, next, g);  // (item counts this one already)
         }
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     auto draw = [&](int idx) {  // tile idx, or the next one that has steps
       DkvItem w(p.d, p.plan, idx, splits, n_items);
       while (CUT && w.there() && !w.steps()) {
-        if (lead) idx = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
+        if (lead) idx = int(gridDim.x) + atomicAdd(p.next + LIST_K, 1);
         w = DkvItem(p.d, p.plan, __shfl_sync(0xffffffffu, idx, 0), splits, n_items);
       }
       return w;
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           }
           if (k == max(w.hi - 3, w.lo)) {
             int idx = 0;
-            if (lead) idx = int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_K], 1);
+            if (lead) idx = int(gridDim.x) + atomicAdd(p.next + LIST_K, 1);
             next = draw(__shfl_sync(0xffffffffu, idx, 0));
             if (lead) feed.put(item, next, g);  // (item counts this one already)
           }
@@ -1031,7 +1032,7 @@ static int launch_packed_bwd(const PackedBwdMaps& maps, const PackedBwdParams& p
 
 extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const void* q, const void* k, const void* v,
                                              const void* o, const void* dO, long long do_row, long long do_head,
-                                             const float* lse2, void* plan, size_t plan_bytes, void* workspace,
+                                             const float* lse2, const void* plan, size_t plan_bytes, void* workspace,
                                              size_t workspace_bytes, void* dq, void* dk, void* dv, int* status,
                                              void* stream) {
   using namespace mea;
@@ -1059,7 +1060,8 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   if (workspace_bytes < packed_backward_bytes(pd))
     return set_error(MEA_ERR_WORKSPACE, "packed attention backward: workspace has %zu bytes, needs %zu", workspace_bytes,
                      packed_backward_bytes(pd));
-  float* delta = static_cast<float*>(workspace);
+  int* next = static_cast<int*>(workspace);
+  float* delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + PACKED_COUNTERS);
   auto st = static_cast<cudaStream_t>(stream);
   if (pd.n_seqs == 0) {  // no sequence owns a row
     if (cudaMemsetAsync(dq, 0, size_t(pd.total) * wq * 2, st) != cudaSuccess ||
@@ -1076,12 +1078,13 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
   if (rc) return set_error(MEA_ERR_CUDA, "packed attention backward: tensor map encode failed (%d)", rc);
   PackedBwdParams p;
   p.d = pd;
-  p.plan = packed_plan_view(pd, plan);
+  p.plan = packed_plan_view(pd, const_cast<void*>(plan));  // read only
   p.scale = d->scale;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.lse2 = lse2;
   p.delta = delta;
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + packed_delta_bytes(pd));
+  p.next = next;
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + PACKED_COUNTERS + packed_delta_bytes(pd));
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
@@ -1091,7 +1094,7 @@ extern "C" int mea_packed_attention_backward(const mea_packed_dims* d, const voi
     return set_error(MEA_ERR_UNSUPPORTED_SHAPE, "packed attention backward: %d rows x %d heads are too many", pd.total, pd.Hq);
   const bool bf = d->dtype == MEA_BF16;
   (bf ? packed_delta_kernel<Bf16> : packed_delta_kernel<Fp16>)<<<unsigned(blocks), 256, 0, st>>>(
-      pd, p.plan.head, static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dO), do_row, do_head, delta,
+      pd, p.plan.head, next, static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dO), do_row, do_head, delta,
       static_cast<uint4*>(dq), static_cast<uint4*>(dk), static_cast<uint4*>(dv));
   if ((rc = check_launch("packed_delta_kernel")) != MEA_OK) return rc;
   if (bf) return pd.N <= 64 ? launch_packed_bwd<64, Bf16>(maps, p, st) : launch_packed_bwd<128, Bf16>(maps, p, st);

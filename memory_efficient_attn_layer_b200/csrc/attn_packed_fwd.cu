@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
               tma_load_3d(sV(sv) + c * 16384, &maps.v, v_raw(sv), c * 64, w.kvh, w.seq0 + j * 128);
             vpar[sv] = int(pv);
             if (j == max(w.n - 3, 0)) {
-              next = FwdItem(p, int(gridDim.x) + atomicAdd(&p.plan.head->next[LIST_FWD], 1), n_items);
+              next = FwdItem(p, int(gridDim.x) + atomicAdd(&p.plan.head->next, 1), n_items);
               feed.put(item + 1, next, g);
             }
           }

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   const bool keys = kind == LIST_K;
   // The sequences in the order they are taken: first row, length, tiles before it.
   const bool in_smem = n_seqs <= PLAN_SMEM_SEQS;
-  int* begin = in_smem ? seq_s : p.scratch + kind * 3 * n_seqs;
+  int* begin = in_smem ? seq_s : p.scratch + size_t(3) * kind * n_seqs;
   int* len = begin + (in_smem ? PLAN_SMEM_SEQS : n_seqs);
   int* pre = len + (in_smem ? PLAN_SMEM_SEQS : n_seqs);
   int longest = 0, most_tiles = 0;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   // output row is then zero) and the status word says so.
   if (!__syncthreads_and(good)) {
     if (tid == 0) {
-      p.plan.head->n[kind] = p.plan.head->next[kind] = 0;
+      p.plan.head->n[kind] = 0;
       if (keys) p.plan.head->splits = 1;
       if (kind == 0) {
         record_error(p.status, KID_PACKED_PLAN, 1);
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) packed_plan_kernel(const int* __
   const int cap = p.d.cap[kind];
   if (tid == 0) {
     p.plan.head->n[kind] = min(n, cap);
-    p.plan.head->next[kind] = 0;
+    if (kind == LIST_FWD) p.plan.head->next = 0;
     if (kind == 0) {
       p.plan.head->first = cu[0];
       p.plan.head->end = cu[n_seqs];
@@ -258,11 +258,10 @@ int packed_dims(const mea_packed_dims* d, PackedDims* out) {
   return MEA_OK;
 }
 
-// Workspace of the backward: delta [total, Hq], then the parts' dK and dV in fp32.
 size_t packed_delta_bytes(const PackedDims& d) { return up256(sizeof(float) * size_t(d.total) * d.Hq); }
 size_t packed_backward_bytes(const PackedDims& d) {
   const size_t parts = d.most_splits > 1 ? size_t(d.most_splits) * 2 * sizeof(float) * d.total * d.Hkv * d.N : 0;
-  return packed_delta_bytes(d) + up256(parts);
+  return PACKED_COUNTERS + packed_delta_bytes(d) + up256(parts);
 }
 
 static size_t plan_scratch(const PackedDims& d) {  // offset of the plan kernel's own space

@@ -329,6 +329,37 @@ def test_captured_call_follows_the_lengths():
     check_device_status(DEV)
 
 
+@pytest.mark.parametrize("lens,hq,hkv", [([300, 1, 128, 2000, 77], 8, 8), ([2500], 8, 1)])
+def test_backward_calls_of_one_forward_at_once(lens, hq, hkv):
+    """Two captured backward calls of one kept forward, replayed on two streams at the same time, again and again: each
+    draws its tiles from counters of its own."""
+    q, k, v, do, cu = _make(lens, hq, hkv, 64, BF, seed=31)
+    want = _run(q, k, v, do, cu)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    cut = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side[0]):  # (a backward runs on its forward's stream, so that one is captured)
+        o = packed_attention(*leaves, cut)
+    torch.cuda.synchronize()
+    graphs = []
+    for s in side:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side[0]):
+            grads = torch.autograd.grad(o, leaves, do, retain_graph=True)
+        graphs.append((graph, s, grads))
+    for _ in range(20):
+        for graph, s, _g in graphs:
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for *_x, grads in graphs:
+            for t, name in zip(grads, ("dq", "dk", "dv")):
+                assert torch.equal(t, want[name]), name
+                t.zero_()
+    check_device_status(DEV)
+
+
 def test_arguments_are_checked():
     q, k, v, do, cu = _make([20], 4, 2, 64, BF)
     cut = torch.tensor(cu, dtype=torch.int32, device=DEV)
