@@ -86,6 +86,9 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     if not grads:
         return torch.tensor(0.0)
     work = [_dense(g) for g in grads]
+    for g, w in zip(grads, work):
+        if g is not w and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+            raise ValueError("a gradient's elements share memory (an expanded tensor), so it cannot be scaled in place")
     idx, arrays = _arrays(work)
     if error_if_nonfinite:
         norm = grad_norm(work, norm_type)

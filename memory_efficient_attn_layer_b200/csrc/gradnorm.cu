@@ -20,6 +20,8 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <memory>
+#include <new>
 
 #include "launch.h"
 #include "ptx.cuh"
@@ -394,6 +396,26 @@ extern "C" int mea_grad_norm(int count, const void* const* grads, const long lon
             static_cast<cudaStream_t>(stream));
 }
 
+// Elements of two tensors at one address would be scaled once or twice as the blocks fall.
+static int gn_apart(int count, void* const* grads, const long long* n, const int* dtypes) {
+  using namespace mea;
+  struct Span {
+    uintptr_t begin, end;
+  };
+  const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[size_t(count) + 1]);
+  if (!spans) return set_error(MEA_ERR_WORKSPACE, "gradient clipping: no host memory for %d tensors", count);
+  int k = 0;
+  for (int i = 0; i < count; ++i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(grads[i]);
+    if (n[i]) spans[k++] = {at, at + uintptr_t(n[i]) * (dtypes[i] == MEA_FP32 ? 4 : 2)};
+  }
+  std::sort(&spans[0], &spans[k], [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (int i = 1; i < k; ++i)
+    if (spans[i].begin < spans[i - 1].end)
+      return set_error(MEA_ERR_INVALID_ARGUMENT, "gradient clipping: two of the tensors overlap in memory");
+  return MEA_OK;
+}
+
 extern "C" int mea_clip_grad_norm(int count, void* const* grads, const long long* n, const int* dtypes, int kind,
                                   double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace mea;
@@ -403,6 +425,7 @@ extern "C" int mea_clip_grad_norm(int count, void* const* grads, const long long
   if (!norm || reinterpret_cast<uintptr_t>(norm) & 3)
     return set_error(MEA_ERR_ALIGNMENT, "gradient clipping: norm must be non-NULL and 4-byte aligned");
   if ((rc = gn_buffers(count, workspace, workspace_bytes)) != MEA_OK) return rc;
+  if ((rc = gn_apart(count, grads, n, dtypes)) != MEA_OK) return rc;
   auto fn = kind == MEA_NORM_INF ? gn_run<true> : gn_run<false>;
   return fn(count, grads, n, dtypes, true, max_norm, norm, nullptr, static_cast<double*>(workspace), gn_cap(count),
             static_cast<cudaStream_t>(stream));

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from gpu_util import DEV
-from memory_efficient_attn_layer_b200 import ShardedAdamW, clip_grad_norm_, grad_norm
+from memory_efficient_attn_layer_b200 import MeaError, ShardedAdamW, clip_grad_norm_, grad_norm
 from oracle.adamw import adamw_step
 
 pytestmark = pytest.mark.gpu
@@ -214,3 +214,16 @@ def test_sharded_adamw_clips(max_norm):
     assert plain.grad_norm is None
     with pytest.raises(ValueError, match="max_grad_norm"):
         ShardedAdamW([torch.nn.Parameter(torch.zeros(8, device=DEV, dtype=BF))], max_grad_norm=-1.0)
+
+
+def test_gradients_that_share_memory_are_refused():
+    buf = torch.randn(300, device=DEV)
+    keep = buf.clone()
+    p, q = (torch.nn.Parameter(torch.zeros(200, device=DEV)) for _ in range(2))
+    p.grad, q.grad = buf[:200], buf[100:]
+    with pytest.raises(MeaError, match="overlap"):
+        clip_grad_norm_([p, q], 1e-3)
+    q.grad = buf[:1].expand(200)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_([p, q], 1e-3)
+    assert torch.equal(buf, keep)
