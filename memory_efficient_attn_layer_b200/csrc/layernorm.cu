@@ -11,9 +11,10 @@
 // backward each thread keeps its own columns for every row that its block takes,
 // so dw and db grow in registers; each block writes one fp32 partial row and a
 // second kernel adds those in a fixed order.  All sums are fp32.  Either way the
-// next rows' loads are in flight while the present ones are summed: 65536 x 2048
-// bf16 takes 92 us forward (5.8 TB/s) and 155 us backward with its column sums
-// (5.2 TB/s); without the second set of rows 106 and 185 us.
+// next rows are on their way while the present ones are summed: forward in
+// registers, backward in shared memory.  65536 x 2048 bf16 takes 92 us forward
+// (5.8 TB/s; 106 us without the second row) and 138 us backward with its column
+// sums (5.8 TB/s; 152 us with the second rows in registers, 185 without).
 //
 // Rows too long for that (above 512 x 8 16-byte vectors forward and 512 x 32
 // elements backward; 16384 and 8192 elements where a row is no whole number of
@@ -27,6 +28,7 @@
 
 #include "launch.h"
 #include "ptx.cuh"
+
 namespace mea {
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -262,9 +264,36 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), ln_fwd_blocks<TPR, VEC * V>
   }
 }
 
+// Asynchronous copies to shared memory; each thread waits for its own.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool live) {  // zeros if not live
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rounds of rows on their way in the backward: a ring of STAGES in shared memory,
+// where every thread puts and finds its own vectors (no barrier), and every warp
+// its rows' statistics.  Between 32 and 64 KB on their way an SM is best, more is
+// slower: 131072 x 1024 bf16, two blocks of 16 KB stages an SM, takes 132 us with
+// two stages, 144 with three, 148 with four; 32768 x 4096, one block of 32 KB
+// stages, 142, 132 and 142.  A row that leaves room for one stage only (16384
+// fp32) still gains by it: 163 us for 4096 rows, 351 through registers that spill.
+// Rows of single elements have the next round in registers.
+template <int VEC, int TPR, int V, int R>
+struct LnRing {
+  static constexpr int THREADS = ln_threads<TPR>(), SLOTS = 2 * R * V;  // 16-byte vectors of a thread and round
+  static constexpr uint32_t ROWS = SLOTS * THREADS * 16, STAGE = ROWS + THREADS / 32 * 2 * R * 4;
+  static constexpr bool USED = VEC > 1;
+  static constexpr int STAGES = !USED || ROWS > 65536 ? 1 : THREADS > 256 && ROWS <= 32768 ? 3 : 2;
+  static constexpr uint32_t BYTES = USED ? STAGES * STAGE : 0;
+};
+
 // R rows per group and round; block i takes every gridDim.x-th round, and the
-// next round's rows are on their way while this one's are summed (they wait as
-// they lie in memory, so the second set costs few registers).  Partial sums of
+// next rounds' rows are on their way while this one's are summed.  Partial sums of
 // the block's rows: part[(2 i) C ..] for dw, part[(2 i + 1) C ..] for db.
 // Columns past C hold dy = 0 and add nothing to any sum.
 template <class T, class W, int VEC, int TPR, int V, int R>
@@ -272,8 +301,11 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
     long long rows, int C, const T* __restrict__ dy, const T* __restrict__ x, const W* __restrict__ w,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part) {
   constexpr int THREADS = ln_threads<TPR>(), GROUPS = THREADS / TPR, PAIRS = V * VEC / 2;
+  using Ring = LnRing<VEC, TPR, V, R>;
+  constexpr bool AGAIN = Ring::USED && V * VEC > 16;  // rows and weights read again for dx, instead of 4 V VEC more registers
   __shared__ float red[2 * 2 * R * THREADS / 32];
-  extern __shared__ float cols[];  // [2][C], only with several groups
+  extern __shared__ __align__(16) char ring[];
+  float* cols = reinterpret_cast<float*>(ring);  // [2][C] at the end, only with several groups
   pdl_launch();
   int turn = 0;
   const int g = threadIdx.x / TPR, lane = threadIdx.x % TPR;
@@ -286,6 +318,8 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
     Row<T, VEC, TPR, V> x[R], d[R];
     float mean[R], rstd[R];
   };
+  const long long step = (long long)gridDim.x * GROUPS * R;
+  long long row0 = (long long)blockIdx.x * GROUPS * R;
   auto fetch = [&](Rows& a, long long row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -297,13 +331,64 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
       a.rstd[r] = live ? rstd_in[row] : 0.f;  // xhat = 0 in rows that are not there
     }
   };
-  const long long step = (long long)gridDim.x * GROUPS * R;
-  long long row0 = (long long)blockIdx.x * GROUPS * R;
+  auto start = [&](int stage, long long row0) {
+    const uint32_t at = smem_u32(ring) + stage * Ring::STAGE + threadIdx.x * 16;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long row = row0 + g * R + r;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = (v * TPR + lane) * VEC;
+        const bool live = row < rows && c < C;
+        const long long from = live ? row * C + c : 0;
+        copy_async16(at + (2 * (r * V + v)) * THREADS * 16, x + from, live);
+        copy_async16(at + (2 * (r * V + v) + 1) * THREADS * 16, dy + from, live);
+      }
+    }
+    const int k = threadIdx.x & 31;
+    if (k < 2 * R) {
+      const long long row = row0 + g * R + (k >> 1);
+      copy_async4(smem_u32(ring) + stage * Ring::STAGE + Ring::ROWS + (threadIdx.x >> 5) * 2 * R * 4 + k * 4,
+                  (k & 1 ? rstd_in : mean_in) + (row < rows ? row : 0), row < rows);
+    }
+    copy_async_commit();
+  };
+  auto collect = [&](Rows& a, int stage) {
+    const char* at = ring + stage * Ring::STAGE;
+    const float* stats = reinterpret_cast<const float*>(at + Ring::ROWS) + (threadIdx.x >> 5) * 2 * R;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const uint4* q = reinterpret_cast<const uint4*>(at) + 2 * (r * V + v) * THREADS + threadIdx.x;
+        if constexpr (Ring::USED) {
+          a.x[r].r[v] = q[0];
+          a.d[r].r[v] = q[THREADS];
+        }
+      }
+      a.mean[r] = stats[2 * r];
+      a.rstd[r] = stats[2 * r + 1];
+    }
+  };
   Rows a;
-  if (row0 < rows) fetch(a, row0);
+  int stage = 0;
+  if constexpr (Ring::USED) {
+#pragma unroll
+    for (int s = 0; s < Ring::STAGES - 1; ++s) start(s, row0 + s * step);
+  } else {
+    if (row0 < rows) fetch(a, row0);
+  }
   for (; row0 < rows; row0 += step) {
     Rows next;
-    if (row0 + step < rows) fetch(next, row0 + step);
+    if constexpr (Ring::USED) {
+      // Into the slot of the round before, which this warp has read.
+      start(stage ? stage - 1 : Ring::STAGES - 1, row0 + (Ring::STAGES - 1) * step);
+      copy_async_wait<Ring::STAGES - 1>();
+      __syncwarp();
+      collect(a, stage);
+    } else if (row0 + step < rows) {
+      fetch(next, row0 + step);
+    }
     float sums[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -321,6 +406,10 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
       sums[2 * r + 1] = s2.x + s2.y;
     }
     group_sum<TPR>(sums, red, turn);
+    if constexpr (AGAIN) {
+      collect(a, stage);
+      load_cols<W, VEC, TPR, V>(w, lane, C, 1.f, ww);
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const long long row = row0 + g * R + r;
@@ -335,7 +424,17 @@ __global__ void __launch_bounds__(ln_threads<TPR>(), 512 / ln_threads<TPR>()) la
       }
       store_row<T, VEC, TPR, V>(dx + row * C, lane, C, o);
     }
-    a = next;
+    if constexpr (Ring::USED) {
+      if constexpr (AGAIN) load_cols<W, VEC, TPR, V>(w, lane, C, 1.f, ww);
+      if (++stage == Ring::STAGES) stage = 0;
+      __syncwarp();  // the statistics are read before a lane copies over them
+    } else {
+      a = next;
+    }
+  }
+  if constexpr (Ring::USED) {
+    copy_async_wait<0>();
+    __syncthreads();  // the ring becomes `cols`
   }
   if (!part) return;
   auto at = [](const float2* f, int i) { return i & 1 ? f[i >> 1].y : f[i >> 1].x; };
@@ -517,9 +616,7 @@ static int ln_bwd_blocks(long long rows, const LnShape& s, int rows_per_round) {
   const long long rounds = (rows + (long long)groups * rows_per_round - 1) / ((long long)groups * rows_per_round);
   return int(std::min<long long>(rounds, std::min(num_sms() * (threads > 256 ? 1 : 2), LN_MAX_PARTS)));
 }
-// Rows per group and round; two rounds are in flight.  Four rows (half as many
-// barriers) spill at 128 registers: 177 against 155 us for 65536 x 2048 bf16, and
-// 226 against 151 us for 262144 x 512.
+// Rows per group and round (131072 x 1024 bf16: two rows 132 us, one 142, four 144).
 template <int VEC, int V>
 constexpr int ln_rows() {
   return VEC * V > 8 ? 1 : 2;
@@ -536,13 +633,21 @@ static void ln_fwd(long long rows, int C, float eps, const void* x, const void* 
       rstd);
 }
 template <class T, class W, int VEC, int TPR, int V>
-static void ln_bwd(long long rows, int C, const void* dy, const void* x, const void* w, const float* mean,
+static int ln_bwd(long long rows, int C, const void* dy, const void* x, const void* w, const float* mean,
                    const float* rstd, void* dx, float* part, int grid, cudaStream_t st) {
   constexpr int THREADS = ln_threads<TPR>();
-  const size_t smem = THREADS > TPR && part ? size_t(2) * C * sizeof(float) : 0;
-  layernorm_bwd_kernel<T, W, VEC, TPR, V, ln_rows<VEC, V>()><<<grid, THREADS, smem, st>>>(
+  auto kernel = layernorm_bwd_kernel<T, W, VEC, TPR, V, ln_rows<VEC, V>()>;
+  // (several groups: the block's sums are joined in [2][C] floats; they fit where a ring was)
+  using Ring = LnRing<VEC, TPR, V, ln_rows<VEC, V>()>;
+  static_assert(Ring::BYTES <= 227 * 1024, "");
+  static_assert(!Ring::USED || THREADS == TPR || Ring::BYTES >= 8u * TPR * V * VEC, "");
+  const size_t smem = Ring::USED ? Ring::BYTES : THREADS > TPR && part ? size_t(2) * C * sizeof(float) : 0;
+  if (Ring::USED && !smem_attr_set(reinterpret_cast<const void*>(kernel), int(Ring::BYTES)))
+    return set_error(MEA_ERR_CUDA, "cudaFuncSetAttribute(layer norm backward) failed");
+  kernel<<<grid, THREADS, smem, st>>>(
       rows, C, static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const W*>(w), mean, rstd,
       static_cast<T*>(dx), part);
+  return check_launch("layernorm_bwd_kernel");
 }
 
 // f(VEC, TPR, V) as compile-time constants for a shape of ln_fwd_shape.
@@ -618,6 +723,7 @@ static int layernorm_bwd(long long rows, int C, const void* dy, const void* x, c
                          cudaStream_t st) {
   int parts = 0;
   if (rows > 0) {
+    int rc = MEA_OK;
     if (s.v == 0) {
       const int grid = int(std::min<long long>(rows, (long long)num_sms() * 2));
       layernorm_bwd_long_kernel<T, W><<<grid, 1024, 0, st>>>(rows, C, static_cast<const T*>(dy), static_cast<const T*>(x),
@@ -627,13 +733,13 @@ static int layernorm_bwd(long long rows, int C, const void* dy, const void* x, c
         layernorm_part_long_kernel<T><<<dim3(unsigned((C + 255) / 256), unsigned(parts)), 256, 0, st>>>(
             rows, C, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, part);
       }
+      rc = check_launch("layernorm_bwd_long_kernel");
     } else {
       parts = ln_bwd_blocks(rows, s, ln_rows_of(s));
       ln_bwd_dispatch<16 / sizeof(T)>(s, [&](auto vec, auto tpr, auto v) {
-        ln_bwd<T, W, vec(), tpr(), v()>(rows, C, dy, x, w, mean, rstd, dx, part, parts, st);
+        rc = ln_bwd<T, W, vec(), tpr(), v()>(rows, C, dy, x, w, mean, rstd, dx, part, parts, st);
       });
     }
-    const int rc = check_launch("layernorm_bwd_kernel");
     if (rc != MEA_OK) return rc;
   }
   if (!part) return MEA_OK;

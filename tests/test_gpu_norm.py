@@ -87,6 +87,13 @@ def test_many_rows(rows):
     _check(x, w, b, 1e-5, dy)
 
 
+@pytest.mark.parametrize("rows,c,dt", [(9500, 512, BF), (4000, 1000, HF), (2500, 2048, BF), (1203, 2048, FP), (1001, 4096, BF),
+                                       (700, 8192, HF), (601, 8192, FP), (600, 16384, BF), (450, 16384, FP)])
+def test_several_rounds_of_every_block(rows, c, dt):
+    """More rows than the blocks take at a time, the last round a part of one: the rings of rows on their way go round."""
+    _check(*_make(rows, c, dt, dt, seed=9)[:3], 1e-5, _make(rows, c, dt, dt, seed=10)[3])
+
+
 @pytest.mark.parametrize("c", [64, 1001, 20001])
 @pytest.mark.parametrize("weight,bias", [(True, False), (False, True), (False, False)])
 def test_without_weight_or_bias(weight, bias, c):
