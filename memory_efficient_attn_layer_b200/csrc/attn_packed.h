@@ -16,6 +16,8 @@ constexpr size_t PACKED_COUNTERS = 256;
 size_t packed_delta_bytes(const PackedDims& d);
 size_t packed_backward_bytes(const PackedDims& d);
 PackedPlan packed_plan_view(const PackedDims& d, void* plan);
+// The rows that a list's tiles walk over are more than half of L2.
+bool packed_wide(const PackedDims& d, int list);
 int run_packed_plan(const PackedDims& d, const int* cu, void* plan, int* status, cudaStream_t st);
 // Pointer, alignment and stride checks of one [total, heads, N] tensor.
 int packed_check_rows(const char* name, const void* base, long long tok, long long head, const PackedDims& d, int heads);

@@ -638,38 +638,38 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
     }
   };
   if (warp < 4) {
-  reg_dealloc<Cfg::REG_REST>();
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
-    const bool lead = lane == 0;
-    const uint32_t box = uint32_t(p.d.p * p.d.tt) * 128 * Tile::NCHUNK;
-    int kvpar[2] = {-1, -1}, qpar[ST];
-    for (int s = 0; s < ST; ++s) qpar[s] = -1;
-    int n = 0, item = 0, raw = 0;
-    auto draw = [&](int idx) {  // tile idx, or the next one that has steps
-      DkvItem w(p.d, p.plan, idx, splits, n_items);
-      while (CUT && w.there() && !w.steps()) {
-        if (lead) idx = int(gridDim.x) + atomicAdd(p.next + LIST_K, 1);
-        w = DkvItem(p.d, p.plan, __shfl_sync(0xffffffffu, idx, 0), splits, n_items);
-      }
-      return w;
-    };
-    DkvItem w = draw(blockIdx.x), next;
-    if (lead) feed.put(0, w, g);
-    while (w.there() && g.ok) {
-      const int kb = item % KVB;
-      if (lead && (item < KVB || mbar_wait(kv_empty(kb), uint32_t((item / KVB - 1) & 1), g, 1))) {
-        mbar_expect_tx(kv_full(kb), 2 * TB);
-#pragma unroll
-        for (int c = 0; c < Tile::NCHUNK; ++c) {
-          tma_load_3d(sK(kb) + c * 16384, &maps.k, kv_full(kb), c * 64, w.kvh, w.seq0 + w.k0);
-          tma_load_3d(sV(kb) + c * 16384, &maps.v, kv_full(kb), c * 64, w.kvh, w.seq0 + w.k0);
+    reg_dealloc<Cfg::REG_REST>();
+    if (warp == 0) {
+      // ---------------- TMA producer ----------------
+      const bool lead = lane == 0;
+      const uint32_t box = uint32_t(p.d.p * p.d.tt) * 128 * Tile::NCHUNK;
+      int kvpar[2] = {-1, -1}, qpar[ST];
+      for (int s = 0; s < ST; ++s) qpar[s] = -1;
+      int n = 0, item = 0, raw = 0;
+      auto draw = [&](int idx) {  // tile idx, or the next one that has steps
+        DkvItem w(p.d, p.plan, idx, splits, n_items);
+        while (CUT && w.there() && !w.steps()) {
+          if (lead) idx = int(gridDim.x) + atomicAdd(p.next + LIST_K, 1);
+          w = DkvItem(p.d, p.plan, __shfl_sync(0xffffffffu, idx, 0), splits, n_items);
         }
-        kvpar[kb] = (item / KVB) & 1;
-      }
-      ++item;
-      DkvStep at(w);
-      for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
+        return w;
+      };
+      DkvItem w = draw(blockIdx.x), next;
+      if (lead) feed.put(0, w, g);
+      while (w.there() && g.ok) {
+        const int kb = item % KVB;
+        if (lead && (item < KVB || mbar_wait(kv_empty(kb), uint32_t((item / KVB - 1) & 1), g, 1))) {
+          mbar_expect_tx(kv_full(kb), 2 * TB);
+#pragma unroll
+          for (int c = 0; c < Tile::NCHUNK; ++c) {
+            tma_load_3d(sK(kb) + c * 16384, &maps.k, kv_full(kb), c * 64, w.kvh, w.seq0 + w.k0);
+            tma_load_3d(sV(kb) + c * 16384, &maps.v, kv_full(kb), c * 64, w.kvh, w.seq0 + w.k0);
+          }
+          kvpar[kb] = (item / KVB) & 1;
+        }
+        ++item;
+        DkvStep at(w);
+        for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
           const int s = n % ST;
           const uint32_t ph = (n / ST) & 1;
           const int t0 = at.qt * p.d.tt;
@@ -706,121 +706,121 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
             if (lead) mbar_arrive(qdo_full(s));
           }
         }
-      w = next;
-    }
-    if (lead) {
-      if (!g.ok) {
-        for (int b = 0; b < KVB; ++b)
-          if (kvpar[b] >= 0) mbar_drain(kv_full(b), uint32_t(kvpar[b]));
-        for (int s = 0; s < ST; ++s)
-          if (qpar[s] >= 0) mbar_drain(qdo_full(s), uint32_t(qpar[s]));
-        mbar_drain(raw_bar, uint32_t(raw & 1));
-      } else {
-        for (int b = 0; b < KVB; ++b)
-          if (kvpar[b] >= 0) mbar_wait(kv_empty(b), uint32_t(kvpar[b]), g, 4);
-        for (int s = 0; s < ST; ++s)
-          if (qpar[s] >= 0) mbar_wait(qdo_empty(s), uint32_t(qpar[s]), g, 5);
+        w = next;
       }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (elect_one()) {
-      bool any = false;
-      // S^T and dP^T run ahead of dV and dK, across items: their next steps.
-      // With two S^T buffers S^T may be an item ahead of dP^T, so the steps of up to
-      // three items in a row are kept (0: no more).
-      int item_steps[3], got = 0;
-      auto steps_of = [&](int item) -> int {
-        while (got <= item) {
-          DkvItem w;
-          const int st = feed.get(got, w, g) ? w.steps() : 0;
-          if (got % 3 == 0) item_steps[0] = st;
-          if (got % 3 == 1) item_steps[1] = st;
-          if (got % 3 == 2) item_steps[2] = st;
-          ++got;
-          if (st == 0) break;
-        }
-        return item % 3 == 0 ? item_steps[0] : item % 3 == 1 ? item_steps[1] : item_steps[2];
-      };
-      struct Ahead {
-        int n, item, left;  // left = 0: no more steps
-      };
-      auto advance = [&](Ahead& a) {
-        ++a.n;
-        if (--a.left == 0) a.left = steps_of(++a.item);
-      };
-      Ahead as{0, 0, steps_of(0)}, ad = as;
-      auto issue_s = [&]() -> bool {  // S^T = K Q^T
-        const int kb = as.item % KVB, s = as.n % ST;
-        if (!mbar_wait(kv_full(kb), (as.item / KVB) & 1, g, 6)) return false;
-        if (!mbar_wait(qdo_full(s), (as.n / ST) & 1, g, 7)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_ss(tmem + Cfg::S_COL + 128 * (as.n % SB), Tile::kmajor(sK(kb), 128, kk), Tile::kmajor(sQ(s), 128, kk),
-                 IDESC_SS, kk > 0 ? 1u : 0u);
-        mma_commit(s_full(as.n % SB));
-        any = true;
-        advance(as);
-        return true;
-      };
-      auto issue_dp = [&]() -> void {  // dP^T = V dO^T, after the same step's S^T: its operands are there
-        const int kb = ad.item % KVB, s = ad.n % ST;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          mma_ss(tmem + Cfg::DP_COL, Tile::kmajor(sV(kb), 128, kk), Tile::kmajor(sdO(s), 128, kk), IDESC_SS,
-                 kk > 0 ? 1u : 0u);
-        mma_commit(dp_full);
-        if (ad.left == 1) mma_commit(kv_empty(kb));  // the item's last read of K and V
-        advance(ad);
-      };
-      int n = 0, item = 0;
-      if (as.left && issue_s()) issue_dp();
-      for (int steps = steps_of(0); steps && g.ok; steps = steps_of(++item)) {
-        for (int k = 0; k < steps; ++k, ++n) {
-          const int s = n % ST;
-          const uint32_t pt = tmem + Cfg::S_COL + 128 * (n % SB), dst = tmem + Cfg::DP_COL;
-          // Two S^T buffers: the next one is free once dV of the step before has been issued.
-          if (SB == 2 && as.left && !issue_s()) break;
-          if (!mbar_wait(p_full(n % SB), (n / SB) & 1, g, 8)) break;
-          if (k == 0 && item > 0 && !mbar_wait(acc_empty, (item - 1) & 1, g, 9)) break;
-          tc_fence_after();
-          // dV += P^T dO: queries [64 hh, 64 hh + 64) of P^T start at column 64 hh.
-#pragma unroll
-          for (int kc = 0; kc < 8; ++kc)
-            mma_ts(tmem + Cfg::DV_COL, pt + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sdO(s), 128, kc), IDESC_KV,
-                   (k > 0 || kc > 0) ? 1u : 0u);
-          // One buffer: after dV, or after the item's last dK, which should not wait for the next K and V.
-          const bool last = k + 1 == steps;
-          if (SB == 1 && as.left && !last && !issue_s()) break;
-          if (!mbar_wait(ds_full, n & 1, g, 10)) break;
-          tc_fence_after();
-          // dK += dS^T Q
-#pragma unroll
-          for (int kc = 0; kc < 8; ++kc)
-            mma_ts(tmem + Cfg::DK_COL, dst + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sQ(s), 128, kc), IDESC_KV,
-                   (k > 0 || kc > 0) ? 1u : 0u);
-          mma_commit(qdo_empty(s));
-          if (last) mma_commit(acc_full);
-          if (SB == 1 && as.left && last && !issue_s()) break;
-          if (ad.left) issue_dp();
+      if (lead) {
+        if (!g.ok) {
+          for (int b = 0; b < KVB; ++b)
+            if (kvpar[b] >= 0) mbar_drain(kv_full(b), uint32_t(kvpar[b]));
+          for (int s = 0; s < ST; ++s)
+            if (qpar[s] >= 0) mbar_drain(qdo_full(s), uint32_t(qpar[s]));
+          mbar_drain(raw_bar, uint32_t(raw & 1));
+        } else {
+          for (int b = 0; b < KVB; ++b)
+            if (kvpar[b] >= 0) mbar_wait(kv_empty(b), uint32_t(kvpar[b]), g, 4);
+          for (int s = 0; s < ST; ++s)
+            if (qpar[s] >= 0) mbar_wait(qdo_empty(s), uint32_t(qpar[s]), g, 5);
         }
       }
-      if (!g.ok && any) {
-        mma_commit(drain_bar);
-        mbar_drain(drain_bar, 0);
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      if (elect_one()) {
+        bool any = false;
+        // S^T and dP^T run ahead of dV and dK, across items: their next steps.
+        // With two S^T buffers S^T may be an item ahead of dP^T, so the steps of up to
+        // three items in a row are kept (0: no more).
+        int item_steps[3], got = 0;
+        auto steps_of = [&](int item) -> int {
+          while (got <= item) {
+            DkvItem w;
+            const int st = feed.get(got, w, g) ? w.steps() : 0;
+            if (got % 3 == 0) item_steps[0] = st;
+            if (got % 3 == 1) item_steps[1] = st;
+            if (got % 3 == 2) item_steps[2] = st;
+            ++got;
+            if (st == 0) break;
+          }
+          return item % 3 == 0 ? item_steps[0] : item % 3 == 1 ? item_steps[1] : item_steps[2];
+        };
+        struct Ahead {
+          int n, item, left;  // left = 0: no more steps
+        };
+        auto advance = [&](Ahead& a) {
+          ++a.n;
+          if (--a.left == 0) a.left = steps_of(++a.item);
+        };
+        Ahead as{0, 0, steps_of(0)}, ad = as;
+        auto issue_s = [&]() -> bool {  // S^T = K Q^T
+          const int kb = as.item % KVB, s = as.n % ST;
+          if (!mbar_wait(kv_full(kb), (as.item / KVB) & 1, g, 6)) return false;
+          if (!mbar_wait(qdo_full(s), (as.n / ST) & 1, g, 7)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            mma_ss(tmem + Cfg::S_COL + 128 * (as.n % SB), Tile::kmajor(sK(kb), 128, kk), Tile::kmajor(sQ(s), 128, kk),
+                   IDESC_SS, kk > 0 ? 1u : 0u);
+          mma_commit(s_full(as.n % SB));
+          any = true;
+          advance(as);
+          return true;
+        };
+        auto issue_dp = [&]() -> void {  // dP^T = V dO^T, after the same step's S^T: its operands are there
+          const int kb = ad.item % KVB, s = ad.n % ST;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            mma_ss(tmem + Cfg::DP_COL, Tile::kmajor(sV(kb), 128, kk), Tile::kmajor(sdO(s), 128, kk), IDESC_SS,
+                   kk > 0 ? 1u : 0u);
+          mma_commit(dp_full);
+          if (ad.left == 1) mma_commit(kv_empty(kb));  // the item's last read of K and V
+          advance(ad);
+        };
+        int n = 0, item = 0;
+        if (as.left && issue_s()) issue_dp();
+        for (int steps = steps_of(0); steps && g.ok; steps = steps_of(++item)) {
+          for (int k = 0; k < steps; ++k, ++n) {
+            const int s = n % ST;
+            const uint32_t pt = tmem + Cfg::S_COL + 128 * (n % SB), dst = tmem + Cfg::DP_COL;
+            // Two S^T buffers: the next one is free once dV of the step before has been issued.
+            if (SB == 2 && as.left && !issue_s()) break;
+            if (!mbar_wait(p_full(n % SB), (n / SB) & 1, g, 8)) break;
+            if (k == 0 && item > 0 && !mbar_wait(acc_empty, (item - 1) & 1, g, 9)) break;
+            tc_fence_after();
+            // dV += P^T dO: queries [64 hh, 64 hh + 64) of P^T start at column 64 hh.
+#pragma unroll
+            for (int kc = 0; kc < 8; ++kc)
+              mma_ts(tmem + Cfg::DV_COL, pt + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sdO(s), 128, kc), IDESC_KV,
+                     (k > 0 || kc > 0) ? 1u : 0u);
+            // One buffer: after dV, or after the item's last dK, which should not wait for the next K and V.
+            const bool last = k + 1 == steps;
+            if (SB == 1 && as.left && !last && !issue_s()) break;
+            if (!mbar_wait(ds_full, n & 1, g, 10)) break;
+            tc_fence_after();
+            // dK += dS^T Q
+#pragma unroll
+            for (int kc = 0; kc < 8; ++kc)
+              mma_ts(tmem + Cfg::DK_COL, dst + (kc >> 2) * 64 + (kc & 3) * 8, Tile::mnmajor(sQ(s), 128, kc), IDESC_KV,
+                     (k > 0 || kc > 0) ? 1u : 0u);
+            mma_commit(qdo_empty(s));
+            if (last) mma_commit(acc_full);
+            if (SB == 1 && as.left && last && !issue_s()) break;
+            if (ad.left) issue_dp();
+          }
+        }
+        if (!g.ok && any) {
+          mma_commit(drain_bar);
+          mbar_drain(drain_bar, 0);
+        }
       }
-    }
-  } else if (warp == 2) {
-    // ---------------- -lse2 and delta of each step's 128 query rows ----------------
-    int n = 0;
-    for (int item = 0; g.ok; ++item) {
-      const volatile DkvItem& slot = *feed.look(item, g);
-      if (!g.ok || !slot.there()) break;
-      const DkvItem w = const_cast<const DkvItem&>(slot);
-      feed.done(item, lane);
-      DkvStep at(w);
-      for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
+    } else if (warp == 2) {
+      // ---------------- -lse2 and delta of each step's 128 query rows ----------------
+      int n = 0;
+      for (int item = 0; g.ok; ++item) {
+        const volatile DkvItem& slot = *feed.look(item, g);
+        if (!g.ok || !slot.there()) break;
+        const DkvItem w = const_cast<const DkvItem&>(slot);
+        feed.done(item, lane);
+        DkvStep at(w);
+        for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
           const int s = n % ST;
           g.ok = __all_sync(0xffffffffu, mbar_wait(qdo_empty(s), ((n / ST) & 1) ^ 1, g, 11));
           if (!g.ok) break;
@@ -835,10 +835,10 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
           }
           mbar_arrive(row_full(s));
         }
+      }
     }
-  }
-  finish();
-  return;
+    finish();
+    return;
   }
   reg_alloc<Cfg::REG_SOFTMAX>();
   {
@@ -859,78 +859,78 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       const int k0 = w.k0, key = k0 + r, qt0 = w.qt0, qt_end = qt0 + w.span;
       int qt = qt0 + w.lo % w.span;
       for (int k = w.hi - w.lo; k > 0; --k, ++n, qt = qt + 1 == qt_end ? qt0 : qt + 1) {
-          const int s = n % ST;
-          ok = __all_sync(0xffffffffu, mbar_wait(row_full(s), (n / ST) & 1, g, 12));
-          if (!ok) break;
-          const int t0 = qt * p.d.tt;
-          const bool mask = t0 < k0 + 127;
-          const int cmin = p.d.p * (key - t0) - 64 * hh;  // first of this thread's columns that sees the key
-          const uint32_t sa = lane_base + Cfg::S_COL + 128 * (n % SB) + 64 * hh;
-          const uint32_t da = lane_base + Cfg::DP_COL + 64 * hh;
-          // The columns' -lse2 and, below, delta come to registers before the waits for
-          // S^T and dP^T: shared memory is busy with the MMAs' operands then.
-          auto row_values = [&](int which, float2(&v)[32]) {
-            const float4* q = reinterpret_cast<const float4*>(rows + s * 256 + 128 * which + 64 * hh);
+        const int s = n % ST;
+        ok = __all_sync(0xffffffffu, mbar_wait(row_full(s), (n / ST) & 1, g, 12));
+        if (!ok) break;
+        const int t0 = qt * p.d.tt;
+        const bool mask = t0 < k0 + 127;
+        const int cmin = p.d.p * (key - t0) - 64 * hh;  // first of this thread's columns that sees the key
+        const uint32_t sa = lane_base + Cfg::S_COL + 128 * (n % SB) + 64 * hh;
+        const uint32_t da = lane_base + Cfg::DP_COL + 64 * hh;
+        // The columns' -lse2 and, below, delta come to registers before the waits for
+        // S^T and dP^T: shared memory is busy with the MMAs' operands then.
+        auto row_values = [&](int which, float2(&v)[32]) {
+          const float4* q = reinterpret_cast<const float4*>(rows + s * 256 + 128 * which + 64 * hh);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float4 f = q[e];
-              v[2 * e] = make_float2(f.x, f.y);
-              v[2 * e + 1] = make_float2(f.z, f.w);
-            }
-          };
-          float2 P[32], rv[32];
-          row_values(0, rv);
-          ok = __all_sync(0xffffffffu, mbar_wait(s_full(n % SB), (n / SB) & 1, g, 13));
-          if (!ok) break;
-          tc_fence_after();
-          tmem_load64(sa, P);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) P[e] = ffma2(P[e], sl2, rv[e]);
-          auto probs = [&](auto masked) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t pk[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                float2 x = exp2_pair(P[8 * c + e], (kPolyPairsBwd >> e) & 1);
-                if (masked()) {
-                  x.x = 16 * c + 2 * e < cmin ? 0.f : x.x;
-                  x.y = 16 * c + 2 * e + 1 < cmin ? 0.f : x.y;
-                }
-                P[8 * c + e] = x;
-                pk[e] = T::pack(x.x, x.y);
-              }
-              tmem_st8(sa + 8 * c, pk);  // over columns this thread has read
-            }
-          };
-          if (mask)
-            probs(std::true_type());
-          else
-            probs(std::false_type());
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(p_full(n % SB));
-          row_values(1, rv);
-          ok = __all_sync(0xffffffffu, mbar_wait(dp_full, n & 1, g, 14));
-          if (!ok) break;
-          tc_fence_after();
-          // (Masked entries have P = 0; keys of other sequences are other lanes, their rows of dO are cleared.)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t dp[32], ds[16];
-            tmem_load32(da + 32 * h, dp);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 x = fmul2(P[16 * h + e], fsub2(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])),
-                                                          rv[16 * h + e]));
-              ds[e] = T::pack(x.x, x.y);
-            }
-            tmem_st16(da + 16 * h, ds);
+          for (int e = 0; e < 16; ++e) {
+            const float4 f = q[e];
+            v[2 * e] = make_float2(f.x, f.y);
+            v[2 * e + 1] = make_float2(f.z, f.w);
           }
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(ds_full);
+        };
+        float2 P[32], rv[32];
+        row_values(0, rv);
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full(n % SB), (n / SB) & 1, g, 13));
+        if (!ok) break;
+        tc_fence_after();
+        tmem_load64(sa, P);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) P[e] = ffma2(P[e], sl2, rv[e]);
+        auto probs = [&](auto masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float2 x = exp2_pair(P[8 * c + e], (kPolyPairsBwd >> e) & 1);
+              if (masked()) {
+                x.x = 16 * c + 2 * e < cmin ? 0.f : x.x;
+                x.y = 16 * c + 2 * e + 1 < cmin ? 0.f : x.y;
+              }
+              P[8 * c + e] = x;
+              pk[e] = T::pack(x.x, x.y);
+            }
+            tmem_st8(sa + 8 * c, pk);  // over columns this thread has read
+          }
+        };
+        if (mask)
+          probs(std::true_type());
+        else
+          probs(std::false_type());
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_full(n % SB));
+        row_values(1, rv);
+        ok = __all_sync(0xffffffffu, mbar_wait(dp_full, n & 1, g, 14));
+        if (!ok) break;
+        tc_fence_after();
+        // (Masked entries have P = 0; keys of other sequences are other lanes, their rows of dO are cleared.)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t dp[32], ds[16];
+          tmem_load32(da + 32 * h, dp);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = fmul2(P[16 * h + e], fsub2(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])),
+                                                        rv[16 * h + e]));
+            ds[e] = T::pack(x.x, x.y);
+          }
+          tmem_st16(da + 16 * h, ds);
         }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(ds_full);
+      }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, mbar_wait(acc_full, item & 1, g, 15));
       if (!ok) break;

@@ -107,7 +107,13 @@ struct FwdItem {
   __device__ bool there() const volatile { return n > 0; }
 };
 
-template <int HD, class T>
+// HALVES: P goes to the MMA warp in two halves of 64 keys, so that PV begins before
+// the last exponentials are through.  Measured (N = 128), whole and in halves:
+// 16384 tokens with 16/2 heads 917 and 867 us, eight ragged prompts with 16/4 heads
+// 69.6 and 67.4; 16 x 2048 tokens with 16/16 heads, the order by sequence (K and V
+// 268 MB), 355 and 366.  So it is taken where the plan goes by work.  At HD = 64 the
+// next scores are computed meanwhile anyway (no change).
+template <int HD, class T, bool HALVES>
 __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constant__ PackedFwdMaps maps,
                                                             const __grid_constant__ PackedFwdParams p) {
   using Cfg = PackedFwdCfg<HD>;
@@ -138,10 +144,11 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
   auto pv_done = [&](int x) { return b0 + 8u * (20 + x); };  // (SEP_P) PV_x(j) done
   auto o_full = [&](int x) { return b0 + 8u * (22 + x); };   // an item's O_x complete
   auto o_empty = [&](int x) { return b0 + 8u * (24 + x); };  // and read out
-  const uint32_t drain_bar = b0 + 8u * 26;
-  const Feed<FwdItem> feed{b0 + 8u * 28, b0 + 8u * 32, reinterpret_cast<FwdItem*>(bars + 42)};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 36);
-  volatile int* bad = reinterpret_cast<int*>(bars + 37);  // per item (mod 4) and stream: V held inf or NaN behind the mask
+  auto p_half = [&](int x) { return b0 + 8u * (26 + x); };   // the first 64 columns of P_x(j) written
+  const uint32_t drain_bar = b0 + 8u * 28;
+  const Feed<FwdItem> feed{b0 + 8u * 29, b0 + 8u * 33, reinterpret_cast<FwdItem*>(bars + 42)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 37);
+  volatile int* bad = reinterpret_cast<int*>(bars + 38);  // per item (mod 4) and stream: V held inf or NaN behind the mask
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -150,6 +157,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_empty(x), 128);
       mbar_init(p_full(x), 128);
+      mbar_init(p_half(x), 128);
       mbar_init(pv_done(x), 1);
       mbar_init(o_full(x), 1);
       mbar_init(o_empty(x), 128);
@@ -281,14 +289,20 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
               if (Cfg::SEP_P && more) {  // the next scores as soon as these are in registers
                 if (!mbar_wait(s_empty(x), done[x] & 1, g, 9) || !issue_s(w, item, k0, x, j + 1)) break;
               }
-              if (!mbar_wait(p_full(x), done[x] & 1, g, 10)) break;
+              if (!mbar_wait(HALVES ? p_half(x) : p_full(x), done[x] & 1, g, 10)) break;
               if (!mbar_wait(v_full(sv), ((k0 + j) / VS) & 1, g, 11)) break;
               if (j == 0 && outs[x] > 0 && !mbar_wait(o_empty(x), (outs[x] - 1) & 1, g, 12)) break;
               tc_fence_after();
 #pragma unroll
-              for (int kc = 0; kc < 8; ++kc)
+              for (int kc = 0; kc < 8; ++kc) {
+                if (HALVES && kc == 4) {
+                  if (!mbar_wait(p_full(x), done[x] & 1, g, 10)) break;
+                  tc_fence_after();
+                }
                 mma_ts(tmem + Cfg::O_COL + HD * x, tmem + Cfg::P_COL + Cfg::P_STEP * x + kc * 8, Tile::mnmajor(sV(sv), 128, kc),
                        IDESC_O, (j > 0 || kc > 0) ? 1u : 0u);
+              }
+              if (!g.ok) break;
               if (Cfg::SEP_P) mma_commit(pv_done(x));
               if (x == 1 || j >= w.nkv[1]) mma_commit(v_empty(sv));
               if (!more) {
@@ -463,6 +477,11 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
               pk[e] = T::pack(pp.x, pp.y);
             }
             tmem_st8(pt + 8 * c, pk);
+            if (HALVES && c == 3) {
+              tmem_st_wait();
+              tc_fence_before();
+              mbar_arrive(p_half(x));
+            }
           }
         };
         if (mask)
@@ -524,7 +543,9 @@ template <int HD, class T>
 static int launch_packed_fwd(const PackedFwdMaps& maps, const PackedFwdParams& p, cudaStream_t st) {
   using Cfg = PackedFwdCfg<HD>;
   static_assert(Cfg::SMEM <= 232448, "shared memory");
-  auto kern = packed_fwd_kernel<HD, T>;
+  // (as the plan kernel decides from the lengths)
+  const bool by_seq = packed_wide(p.d, LIST_FWD) && (long long)p.d.total / p.d.rows[LIST_FWD] * p.d.hg >= 8LL * num_sms();
+  auto kern = HD <= 64 || by_seq ? packed_fwd_kernel<HD, T, false> : packed_fwd_kernel<HD, T, (HD > 64)>;
   if (!smem_attr_set(reinterpret_cast<const void*>(kern), int(Cfg::SMEM)))
     return set_error(MEA_ERR_CUDA, "cudaFuncSetAttribute(packed_fwd) failed");
   cudaLaunchAttribute attr;

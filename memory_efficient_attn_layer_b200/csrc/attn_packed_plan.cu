@@ -286,15 +286,17 @@ PackedPlan packed_plan_view(const PackedDims& d, void* plan) {
   return v;
 }
 
+bool packed_wide(const PackedDims& d, int list) {  // Q and dO, or K and V
+  return 4LL * d.total * (list == LIST_K ? d.Hq : d.Hkv) * d.N > (64LL << 20);
+}
+
 int run_packed_plan(const PackedDims& d, const int* cu, void* plan, int* status, cudaStream_t st) {
   PlanParams p;
   p.d = d;
   p.plan = packed_plan_view(d, plan);
-  constexpr long long kHalfL2 = 64LL << 20;
-  const bool wide_kv = 4LL * d.total * d.Hkv * d.N > kHalfL2, wide_q = 4LL * d.total * d.Hq * d.N > kHalfL2;
   for (int i = 0; i < 3; ++i) {
     p.at_once[i] = num_sms() / d.heads[i];
-    p.wide[i] = i == LIST_K ? wide_q : wide_kv;  // Q and dO, or K and V
+    p.wide[i] = packed_wide(d, i);
   }
   p.scratch = reinterpret_cast<int*>(static_cast<char*>(plan) + plan_scratch(d));
   p.status = status;
