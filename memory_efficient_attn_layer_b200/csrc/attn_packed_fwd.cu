@@ -15,6 +15,15 @@
 // over S (S_0 S_1 O_0 O_1); HD = 64 has columns for P, so the next scores are
 // computed as soon as these are in registers.
 //
+// What bounds it: at HD = 128 the chain of one stream's step (scores, maximum and
+// exponentials about 1900 clocks, then 1024 of MMAs and their hand-overs), which
+// the other stream hides in part (tensor pipe 61 to 66% busy); at HD = 64, where a
+// step has half the MMA work, the exponentials (three in eight of them as a
+// polynomial on the FMA pipe).  16384 tokens with 16/2 heads of 128: 870 us, 1.25
+// PF/s; with 8/8 heads of 64: 410 us; 16 documents of 21267 tokens, 8/8 heads of
+// 64: 84 us.  One query tile to a CTA and eight softmax warps took 1320 us and more
+// for the first.
+//
 // Rows of other sequences never reach a result: the last key tile's V rows past
 // the sequence's end are cleared in shared memory (their P is zero, but zero
 // times an inf or NaN is not), and so are the inf or NaN elements of V in the
