@@ -18,10 +18,10 @@
 // What bounds it: at HD = 128 the chain of one stream's step (scores, maximum and
 // exponentials about 1900 clocks, then 1024 of MMAs and their hand-overs), which
 // the other stream hides in part (tensor pipe 61 to 66% busy); at HD = 64, where a
-// step has half the MMA work, the exponentials (three in eight of them as a
-// polynomial on the FMA pipe).  16384 tokens with 16/2 heads of 128: 870 us, 1.25
-// PF/s; with 8/8 heads of 64: 410 us; 16 documents of 21267 tokens, 8/8 heads of
-// 64: 84 us.  One query tile to a CTA and eight softmax warps took 1320 us and more
+// step has half the MMA work, the exponentials (a quarter of them as a
+// polynomial on the FMA pipe).  16384 tokens with 16/2 heads of 128: 865 us, 1.27
+// PF/s; with 8/8 heads of 64: 385 us; 16 documents of 21267 tokens, 8/8 heads of
+// 64: 81 us.  One query tile to a CTA and eight softmax warps took 1320 us and more
 // for the first.
 //
 // Rows of other sequences never reach a result: the last key tile's V rows past
@@ -61,6 +61,11 @@ struct PackedFwdCfg {
   static constexpr uint32_t OFF_K = QB * 2 * TB, OFF_V = OFF_K + KS * TB, OFF_BAR = OFF_V + VS * TB;
   static constexpr uint32_t OFF_OUT = OFF_BAR + 768;
   static constexpr size_t SMEM = 1024 + OFF_OUT + 8 * WarpRows<(HD > 64)>::BYTES;
+  // Which of eight pairs of exponentials run on the FMA pipe: a quarter, where the
+  // other attention kernels' share is three eighths (16384 tokens with 8/8 heads of
+  // 64: 384 us, three eighths 410, half 438, none 418; 16/2 heads of 128: 865, 881,
+  // 950, 904).
+  static constexpr uint32_t POLY_PAIRS = HD <= 64 ? 0x44 : 0x42;
   static constexpr int REG_SOFTMAX = 208, REG_REST = 88;  // 256 x 208 + 128 x 88 = 384 x 168
 };
 
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float2 pp = exp2_pair(ffma2(make_float2(s[16 * c + 2 * e], s[16 * c + 2 * e + 1]), sl2, neg_m),
-                                          !masked() && ((kPolyPairsFwd >> e) & 1));
+                                          !masked() && ((Cfg::POLY_PAIRS >> e) & 1));
               if (e & 1)
                 acc1 = fadd2(acc1, pp);
               else
