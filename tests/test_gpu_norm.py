@@ -88,10 +88,21 @@ def test_many_rows(rows):
 
 
 @pytest.mark.parametrize("rows,c,dt", [(9500, 512, BF), (4000, 1000, HF), (2500, 2048, BF), (1203, 2048, FP), (1001, 4096, BF),
-                                       (700, 8192, HF), (601, 8192, FP), (600, 16384, BF), (450, 16384, FP)])
+                                       (700, 8192, HF), (601, 8192, FP), (600, 16384, BF), (450, 16384, FP),
+                                       (20003, 17, BF), (9001, 100, HF), (9003, 333, FP), (6007, 1001, BF), (2501, 2047, HF),
+                                       (1501, 4090, BF), (1201, 3001, FP), (1103, 6001, BF), (701, 8177, HF)])
 def test_several_rounds_of_every_block(rows, c, dt):
     """More rows than the blocks take at a time, the last round a part of one: the rings of rows on their way go round."""
     _check(*_make(rows, c, dt, dt, seed=9)[:3], 1e-5, _make(rows, c, dt, dt, seed=10)[3])
+
+
+@pytest.mark.parametrize("c,dt", [(16, BF), (17, BF), (23, HF), (31, BF), (9, FP), (11, FP), (4081, BF), (4082, HF), (8178, BF),
+                                  (8185, BF), (4089, FP), (4093, FP)])
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9])
+def test_widths_at_the_limits_of_the_vectors(rows, c, dt):
+    """Rows at every alignment within 16 bytes, few of each."""
+    x, w, b, dy = _make(rows, c, dt, dt, seed=rows * c)
+    _check(x, w, b, 1e-5, dy)
 
 
 @pytest.mark.parametrize("c", [64, 1001, 20001])
