@@ -94,6 +94,12 @@ def test_many_sequences():
     _check(lens, 2, 1, 64, BF, seed=9)
 
 
+@pytest.mark.parametrize("n,hq,hkv", [(128, 8, 8), (128, 16, 8), (64, 16, 16)])
+def test_tiles_taken_by_sequence(n, hq, hkv):
+    """K and V beyond half of L2 and many tiles: sequence after sequence instead of the longest tiles first."""
+    _check([300, 257, 0, 256, 310] * 30 + [1000, 1, 2000, 700], hq, hkv, n, BF, seed=17, behind=7)
+
+
 @pytest.mark.parametrize("dt", [BF, HF])
 def test_scale_and_large_scores(dt):
     _check([190, 40], 2, 2, 64, dt, scale=0.5, seed=2)
