@@ -37,6 +37,7 @@ struct PackedHeader {
 struct PackedDims {
   int total, n_seqs, Hq, Hkv, N;
   int p, tt;        // heads and tokens of a query tile
+  int p_inv;        // ceil(2^16 / p)
   int hg;           // query tiles per token tile: Hq / p
   int streams;      // query tiles of a forward item
   int rows[3];      // tokens of a tile of each list
@@ -44,6 +45,9 @@ struct PackedDims {
   int cap[3];       // entries there can be
   int most_splits;  // parts that a key tile's walk may be cut into
 };
+
+// The token of a query tile's row: row / p, exact for rows below 128.
+__device__ __forceinline__ int token_of(const PackedDims& d, int row) { return row * d.p_inv >> 16; }
 
 enum PackedList { LIST_Q = 0, LIST_K = 1, LIST_FWD = 2 };
 struct PackedPlan {

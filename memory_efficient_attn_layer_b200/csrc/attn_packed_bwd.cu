@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (uint32_t(quarter * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    const int tok = r / p.d.p, hr = r - tok * p.d.p;
+    const int tok = token_of(p.d, r), hr = r - tok * p.d.p;
     WarpRows<true> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<true>::BYTES, lane, quarter * 32);
     bool ok = true;
     int n = 0, item = 0;
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
       mbar_arrive(dq_empty);
 #pragma unroll
       for (int i = 0; i < out.rows(); ++i) {
-        const int row_tok = out.row(i) / p.d.p;
+        const int row_tok = token_of(p.d, out.row(i));
         out.off[i] = (row_tok * p.d.Hq + out.row(i) - row_tok * p.d.p) * p.d.N;
         out.live[i] = row_tok < w.t1 - t0;
       }
@@ -819,6 +819,13 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
       }
     } else if (warp == 2) {
       // ---------------- -lse2 and delta of each step's 128 query rows ----------------
+      // (in registers while the stage is still in use)
+      int tok[4], head[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        tok[i] = token_of(p.d, lane + 32 * i);
+        head[i] = lane + 32 * i - tok[i] * p.d.p;
+      }
       int n = 0;
       for (int item = 0; g.ok; ++item) {
         const volatile DkvItem& slot = *feed.look(item, g);
@@ -826,20 +833,30 @@ __global__ void __launch_bounds__(384, 1) packed_dkv_kernel(const __grid_constan
         const DkvItem w = const_cast<const DkvItem&>(slot);
         feed.done(item, lane);
         DkvStep at(w);
-        for (int k = w.lo; k < w.hi; ++k, ++n, at.next(w)) {
+        float l[4], d[4];
+        auto fetch = [&]() {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = at.qt * p.d.tt + tok[i];
+            const bool live = tok[i] < p.d.tt && t < w.len;
+            const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + at.gi * p.d.p + head[i];
+            l[i] = live ? -__ldg(p.lse2 + row) : -INFINITY;  // P = 0 in rows that are not there
+            d[i] = live ? p.delta[row] : 0.f;
+          }
+        };
+        if (w.lo < w.hi) fetch();
+        for (int k = w.lo; k < w.hi; ++k, ++n) {
           const int s = n % ST;
           g.ok = __all_sync(0xffffffffu, mbar_wait(qdo_empty(s), ((n / ST) & 1) ^ 1, g, 11));
           if (!g.ok) break;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = lane + 32 * i;
-            const int tok = r / p.d.p, t = at.qt * p.d.tt + tok;
-            const bool live = tok < p.d.tt && t < w.len;
-            const long long row = (long long)(w.seq0 + t) * p.d.Hq + w.h0 + at.gi * p.d.p + (r - tok * p.d.p);
-            rows[s * 256 + r] = live ? -__ldg(p.lse2 + row) : -INFINITY;  // P = 0 in rows that are not there
-            rows[s * 256 + 128 + r] = live ? p.delta[row] : 0.f;
+            rows[s * 256 + lane + 32 * i] = l[i];
+            rows[s * 256 + 128 + lane + 32 * i] = d[i];
           }
           mbar_arrive(row_full(s));
+          at.next(w);
+          if (k + 1 < w.hi) fetch();
         }
       }
     }

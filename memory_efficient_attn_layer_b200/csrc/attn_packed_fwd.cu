@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
                  gridDim.x, threadIdx.x - 128, 256);
     const int x = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;
-    const int tok = r / p.d.p;
+    const int tok = token_of(p.d, r);
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t st = lane_base + Cfg::S_COL + 128 * x, pt = lane_base + Cfg::P_COL + Cfg::P_STEP * x;
     const uint32_t ot = lane_base + Cfg::O_COL + HD * x;
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(384, 1) packed_fwd_kernel(const __grid_constan
       WarpRows<(HD > 64)> out(base + Cfg::OFF_OUT + (warp - 4) * WarpRows<(HD > 64)>::BYTES, lane, (warp & 3) * 32);
 #pragma unroll
       for (int i = 0; i < out.rows(); ++i) {
-        const int row_tok = out.row(i) / p.d.p;
+        const int row_tok = token_of(p.d, out.row(i));
         out.off[i] = (row_tok * p.d.Hq + out.row(i) - row_tok * p.d.p) * p.d.N;
         out.live[i] = row_tok < min(p.d.tt, w.end - first);
       }

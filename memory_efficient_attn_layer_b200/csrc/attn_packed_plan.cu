@@ -236,6 +236,7 @@ int packed_dims(const mea_packed_dims* d, PackedDims* out) {
       o.p = p;
       o.tt = 128 / p;
     }
+  o.p_inv = (65536 + o.p - 1) / o.p;
   o.hg = d->Hq / o.p;
   // Two query tiles to a forward item where that still gives every SM one.
   o.streams = (long long)d->total / (2 * o.tt) * o.hg >= num_sms() ? 2 : 1;
