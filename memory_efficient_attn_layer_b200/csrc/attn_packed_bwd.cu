@@ -23,11 +23,11 @@
 // queries is cut into parts that leave fp32 partial sums, added in their order by
 // packed_dkv_sum_kernel.
 //
-// What bounds it: the MMAs, at 1.1 to 1.2 PF/s (55 to 60% of the tensor pipe; S and
+// What bounds it: the MMAs, at 1.2 to 1.3 PF/s (about 60% of the tensor pipe; S and
 // dP read both operands from shared memory at its full rate), and at HD = 64 the
 // exponentials beside MMAs of half the work.  12289 + 4095 tokens with 16/4 heads of
-// 128: dQ 830 us, dK/dV 1160 us; 16 documents of 21267 tokens with 8/8 heads of 64:
-// dQ 105 us, dK/dV 141 us; delta 14 us (HBM).
+// 128: dQ 830 us, dK/dV 1060 us; 16 documents of 21267 tokens with 8/8 heads of 64:
+// dQ 104 us, dK/dV 128 us; delta 14 us (HBM).
 //
 // Warps (384 threads, persistent, one CTA per SM): 0 TMA, 1 MMA issue, 2 (dK/dV)
 // lse2 and delta rows, 4..11 softmax: two warps per TMEM lane quarter, half a row
