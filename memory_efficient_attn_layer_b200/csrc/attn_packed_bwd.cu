@@ -23,10 +23,10 @@
 // queries is cut into parts that leave fp32 partial sums, added in their order by
 // packed_dkv_sum_kernel.
 //
-// What bounds it: the MMAs, at 1.2 to 1.3 PF/s (about 60% of the tensor pipe; S and
+// What bounds it: the MMAs, at 1.2 to 1.4 PF/s (60 to 72% of the tensor pipe; S and
 // dP read both operands from shared memory at its full rate), and at HD = 64 the
 // exponentials beside MMAs of half the work.  12289 + 4095 tokens with 16/4 heads of
-// 128: dQ 830 us, dK/dV 1060 us; 16 documents of 21267 tokens with 8/8 heads of 64:
+// 128: dQ 874 us, dK/dV 1003 us; 16 documents of 21267 tokens with 8/8 heads of 64:
 // dQ 104 us, dK/dV 128 us; delta 14 us (HBM).
 //
 // Warps (384 threads, persistent, one CTA per SM): 0 TMA, 1 MMA issue, 2 (dK/dV)
@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(384, 1) packed_dq_kernel(const __grid_constant
           const bool more = nkv1 > 0;
           if (j + 1 == nkv) nkv_next = nkv1;  // the lookahead stands at the next item by now
           // With one Q/dO buffer the next item's rows arrive late: this item's last dQ goes first.
+          // (dP behind dQ: before it, 16384 tokens with 16/2 heads take 1419 us instead of 1272.)
           const bool early = more && (QB == 2 || j + 1 < nkv);
           if (early && !(mbar_wait(s_empty, n & 1, g, 11) && issue_s())) break;
           if (!mbar_wait(ds_full, n & 1, g, 13)) break;
